@@ -7,10 +7,11 @@ callers; C/C++ callers use include/cottus_b200.h directly.
 """
 from ._lib import (COTTUS_ERR_CUDA, COTTUS_ERR_DOUBLE_FREE, COTTUS_ERR_INVALID_ARGUMENT, COTTUS_ERR_OUT_OF_MEMORY,
                    COTTUS_ERR_OUT_OF_RANGE, COTTUS_ERR_UNSUPPORTED, COTTUS_ERR_WORKSPACE, COTTUS_OK, LIB_PATH,
-                   STATUS_BAD_BLOCK_ID, STATUS_BAD_CONTEXT, STATUS_BAD_POSITION, STATUS_TIMEOUT, CottusError, lib)
-from .ops import (BlockAllocator, DecodeBatch, attention_block, lse_combine, o_proj_residual, paged_decode, paged_gather,
-                  qkv_rope_append, rope,
-                  rope_append, rope_append_decode, rope_cos_sin_table)
+                   STATUS_BAD_BLOCK_ID, STATUS_BAD_CONTEXT, STATUS_BAD_POSITION, STATUS_NO_TOKEN, STATUS_TIMEOUT,
+                   CottusError, lib)
+from .ops import (BlockAllocator, DecodeBatch, attention_block, fp8_linear, lse_combine, o_proj_residual, paged_decode,
+                  paged_gather, qkv_rope_append, quantize_fp8, rms_norm, rope, rope_append, rope_append_decode,
+                  rope_cos_sin_table, sample_tokens)
 
 __all__ = [
     "BlockAllocator", "CottusError", "attention_block", "DecodeBatch", "LIB_PATH", "lib", "lse_combine", "o_proj_residual", "paged_decode", "paged_gather",
@@ -19,4 +20,5 @@ __all__ = [
     "COTTUS_ERR_OUT_OF_RANGE", "COTTUS_ERR_CUDA", "COTTUS_ERR_UNSUPPORTED", "COTTUS_ERR_WORKSPACE",
     "COTTUS_ERR_OUT_OF_MEMORY", "COTTUS_ERR_DOUBLE_FREE", "STATUS_BAD_BLOCK_ID", "STATUS_BAD_CONTEXT",
     "STATUS_BAD_POSITION", "STATUS_TIMEOUT",
+    "STATUS_NO_TOKEN", "fp8_linear", "quantize_fp8", "rms_norm", "sample_tokens",
 ]

@@ -25,8 +25,9 @@ STATUS_BAD_BLOCK_ID = 0x1
 STATUS_BAD_CONTEXT = 0x2
 STATUS_BAD_POSITION = 0x4
 STATUS_TIMEOUT = 0x8
+STATUS_NO_TOKEN = 0x10
 
-F32, F16 = 0, 1
+F32, F16, BF16, E4M3 = 0, 1, 2, 3
 
 _vp, _i32, _i64, _f32, _sz = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_size_t
 
@@ -87,6 +88,35 @@ class OProjParams(C.Structure):
     ]
 
 
+class RmsNormParams(C.Structure):
+    _fields_ = [
+        ("x", _vp), ("residual", _vp), ("residual_out", _vp), ("weight", _vp), ("out", _vp), ("scales", _vp),
+        ("rows", _i64), ("hidden", _i32), ("x_dtype", _i32), ("out_dtype", _i32), ("eps", _f32),
+    ]
+
+
+class QuantizeParams(C.Structure):
+    _fields_ = [
+        ("x", _vp), ("out", _vp), ("scales", _vp),
+        ("rows", _i64), ("cols", _i32), ("x_dtype", _i32), ("block_rows", _i32),
+    ]
+
+
+class Fp8LinearParams(C.Structure):
+    _fields_ = [
+        ("x", _vp), ("x_scales", _vp), ("weight", _vp), ("w_scales", _vp), ("residual", _vp), ("out", _vp),
+        ("rows", _i32), ("out_features", _i32), ("in_features", _i32), ("out_dtype", _i32), ("status", _vp),
+    ]
+
+
+class SampleParams(C.Structure):
+    _fields_ = [
+        ("logits", _vp), ("uniforms", _vp), ("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp),
+        ("tokens", _vp), ("logprobs", _vp),
+        ("batch", _i32), ("vocab", _i32), ("dtype", _i32), ("status", _vp),
+    ]
+
+
 class CottusError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"{message} (code {code})")
@@ -131,6 +161,10 @@ def lib() -> C.CDLL:
         ("cottus_qkv_rope_append", C.c_int, [P(QkvParams), _vp]),
         ("cottus_o_proj_residual_workspace_size", _sz, [P(OProjParams)]),
         ("cottus_o_proj_residual", C.c_int, [P(OProjParams), _vp]),
+        ("cottus_rms_norm", C.c_int, [P(RmsNormParams), _vp]),
+        ("cottus_quantize_fp8", C.c_int, [P(QuantizeParams), _vp]),
+        ("cottus_fp8_linear", C.c_int, [P(Fp8LinearParams), _vp]),
+        ("cottus_sample_tokens", C.c_int, [P(SampleParams), _vp]),
         ("cottus_peer_exchange_create", C.c_int, [_i32, _i32, _i32, _i32, _i32, P(_vp), _vp]),
         ("cottus_peer_exchange_open", C.c_int, [_vp, _vp]),
         ("cottus_peer_exchange_set_wait_cycles", C.c_int, [_vp, _i64]),

@@ -11,10 +11,13 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import (F16, F32, CottusError, DecodeBatchDesc, DecodeStepParams, LseCombineParams, PagedDecodeParams,
-                   OProjParams, QkvParams, check, lib)
+from ._lib import (BF16, E4M3, F16, F32, CottusError, DecodeBatchDesc, DecodeStepParams, Fp8LinearParams,
+                   LseCombineParams, PagedDecodeParams, OProjParams, QkvParams, QuantizeParams, RmsNormParams,
+                   SampleParams, check, lib)
 
 _DT = {torch.float32: F32, torch.float16: F16}
+_FP8 = torch.float8_e4m3fn
+_DT_WIDE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}  # norm, 8-bit and sampling operators
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -283,6 +286,151 @@ def attention_block(batch, x, w_qkv, w_o, residual, kv_pool, cos_sin, *, num_hea
     att = att_out.view(n, num_heads * head_dim)
     o_proj_residual(att, w_o, residual, out=residual, status=status, stream=stream)
     return att
+
+
+def _operand(t: torch.Tensor, name: str, shape, dtypes, device: int) -> int:
+    """Checks one operand of the norm, 8-bit and sampling operators; its address."""
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on cuda:{t.get_device()}, the current device is cuda:{device}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+_ONLY_F32, _ONLY_I32, _ONLY_FP8 = (torch.float32,), (torch.int32,), (_FP8,)
+
+
+def rms_norm(x, weight, *, eps=1e-5, residual=None, residual_out=None, out=None, out_dtype=None, scales=None,
+             stream=None):
+    """RMS norm with the residual's addition (cottus_rms_norm):
+    h = x (+ residual), y = h / sqrt(mean(h^2) + eps) * weight.
+
+    x [rows][hidden] fp32, fp16 or bf16; weight [hidden] fp32; residual [rows][hidden] fp32, replaced by h
+    (or h goes to residual_out).  out_dtype defaults to x's.  Returns y, or, with out_dtype
+    torch.float8_e4m3fn, (y, scales): scales [ceil(hidden / 128)][rows] fp32, y = values * their group's scale."""
+    if x.dim() != 2:
+        raise ValueError("x must be [rows][hidden]")
+    dev = torch.cuda.current_device()
+    rows, hidden = x.shape
+    p = RmsNormParams()
+    p.x = _operand(x, "x", x.shape, _DT_WIDE, dev)
+    p.weight = _operand(weight, "weight", (hidden,), _ONLY_F32, dev)
+    if residual is not None:
+        p.residual = _operand(residual, "residual", x.shape, _ONLY_F32, dev)
+        p.residual_out = p.residual if residual_out is None else _operand(residual_out, "residual_out", x.shape,
+                                                                          _ONLY_F32, dev)
+    elif residual_out is not None:
+        raise ValueError("residual_out goes with residual")
+    if out is None:
+        out = torch.empty((rows, hidden), dtype=out_dtype or x.dtype, device=x.device)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise TypeError(f"out is {out.dtype}, out_dtype is {out_dtype}")
+    fp8 = out.dtype == _FP8
+    p.out = _operand(out, "out", x.shape, _ONLY_FP8 if fp8 else _DT_WIDE, dev)
+    if fp8:
+        if scales is None:
+            scales = torch.empty(((hidden + 127) // 128, rows), dtype=torch.float32, device=x.device)
+        p.scales = _operand(scales, "scales", ((hidden + 127) // 128, rows), _ONLY_F32, dev)
+    elif scales is not None:
+        raise ValueError("scales go with a torch.float8_e4m3fn output")
+    p.rows, p.hidden, p.x_dtype, p.out_dtype = rows, hidden, _DT_WIDE[x.dtype], E4M3 if fp8 else _DT_WIDE[out.dtype]
+    p.eps = eps
+    check(lib().cottus_rms_norm(C.byref(p), _stream(stream)))
+    return (out, scales) if fp8 else out
+
+
+def quantize_fp8(x, *, block_rows=1, out=None, scales=None, stream=None):
+    """x [rows][cols] (fp32, fp16, bf16) in e4m3 with fp32 scales (cottus_quantize_fp8): (values, scales).
+    block_rows 1: the activations of fp8_linear, one scale per row and 128 columns, [ceil(cols / 128)][rows];
+    block_rows 128: its weight, one scale per 128 x 128 block, [ceil(rows / 128)][ceil(cols / 128)]."""
+    if x.dim() != 2:
+        raise ValueError("x must be [rows][cols]")
+    dev = torch.cuda.current_device()
+    rows, cols = x.shape
+    p = QuantizeParams()
+    p.x = _operand(x, "x", x.shape, _DT_WIDE, dev)
+    if out is None:
+        out = torch.empty((rows, cols), dtype=_FP8, device=x.device)
+    groups = (cols + 127) // 128
+    shape = ((rows + 127) // 128, groups) if block_rows == 128 else (groups, rows)
+    if scales is None:
+        scales = torch.empty(shape, dtype=torch.float32, device=x.device)
+    p.out = _operand(out, "out", x.shape, _ONLY_FP8, dev)
+    p.scales = _operand(scales, "scales", shape, _ONLY_F32, dev)
+    p.rows, p.cols, p.x_dtype, p.block_rows = rows, cols, _DT_WIDE[x.dtype], block_rows
+    check(lib().cottus_quantize_fp8(C.byref(p), _stream(stream)))
+    return out, scales
+
+
+def fp8_linear(x, x_scales, weight, weight_scales, *, residual=None, out=None, out_dtype=torch.float16, status=None,
+               stream=None):
+    """Block-scaled e4m3 product (cottus_fp8_linear): out = x . weight^T (+ residual), fp32 accumulation.
+    x [rows][in] and x_scales from rms_norm or quantize_fp8; weight [out][in] and weight_scales from
+    quantize_fp8(block_rows=128); residual [rows][out] fp32 (may be out itself where out is fp32).
+    in a multiple of 16."""
+    if x.dim() != 2 or weight.dim() != 2:
+        raise ValueError("x must be [rows][in] and weight [out][in]")
+    dev = torch.cuda.current_device()
+    (rows, fin), fout = x.shape, weight.shape[0]
+    groups = (fin + 127) // 128
+    p = Fp8LinearParams()
+    p.x = _operand(x, "x", x.shape, _ONLY_FP8, dev)
+    p.x_scales = _operand(x_scales, "x_scales", (groups, rows), _ONLY_F32, dev)
+    p.weight = _operand(weight, "weight", (fout, fin), _ONLY_FP8, dev)
+    p.w_scales = _operand(weight_scales, "weight_scales", ((fout + 127) // 128, groups), _ONLY_F32, dev)
+    if residual is not None:
+        p.residual = _operand(residual, "residual", (rows, fout), _ONLY_F32, dev)
+    if out is None:
+        out = torch.empty((rows, fout), dtype=out_dtype, device=x.device)
+    p.out = _operand(out, "out", (rows, fout), _DT_WIDE, dev)
+    p.rows, p.out_features, p.in_features, p.out_dtype = rows, fout, fin, _DT_WIDE[out.dtype]
+    if status is not None:
+        p.status = _operand(status, "status", (1,), _ONLY_I32, dev)
+    check(lib().cottus_fp8_linear(C.byref(p), _stream(stream)))
+    return out
+
+
+def sample_tokens(logits, uniforms, *, temperature=None, top_k=None, top_p=None, min_p=None, out=None,
+                  return_logprobs=False, logprobs=None, status=None, stream=None):
+    """One token per row of logits [batch][vocab] (cottus_sample_tokens) from uniforms [batch] in [0, 1):
+    temperature, then top-k, top-p and min-p, then the inverse of the running sum in index order.
+    temperature, top_p and min_p are fp32 [batch], top_k int32 [batch]; None leaves a filter off
+    (temperature: 1; a row with temperature 0 takes its largest logit).  Returns tokens int32 [batch] (-1 for a row
+    without a finite logit), or (tokens, logprobs fp32 [batch]) with return_logprobs."""
+    if logits.dim() != 2:
+        raise ValueError("logits must be [batch][vocab]")
+    dev = torch.cuda.current_device()
+    batch, vocab = logits.shape
+    row = (batch,)
+    p = SampleParams()
+    p.logits = _operand(logits, "logits", logits.shape, _DT_WIDE, dev)
+    p.uniforms = _operand(uniforms, "uniforms", row, _ONLY_F32, dev)
+    if temperature is not None:
+        p.temperature = _operand(temperature, "temperature", row, _ONLY_F32, dev)
+    if top_k is not None:
+        p.top_k = _operand(top_k, "top_k", row, _ONLY_I32, dev)
+    if top_p is not None:
+        p.top_p = _operand(top_p, "top_p", row, _ONLY_F32, dev)
+    if min_p is not None:
+        p.min_p = _operand(min_p, "min_p", row, _ONLY_F32, dev)
+    if out is None:
+        out = torch.empty(row, dtype=torch.int32, device=logits.device)
+    p.tokens = _operand(out, "out", row, _ONLY_I32, dev)
+    if return_logprobs and logprobs is None:
+        logprobs = torch.empty(row, dtype=torch.float32, device=logits.device)
+    if logprobs is not None:
+        p.logprobs = _operand(logprobs, "logprobs", row, _ONLY_F32, dev)
+    if status is not None:
+        p.status = _operand(status, "status", (1,), _ONLY_I32, dev)
+    p.batch, p.vocab, p.dtype = batch, vocab, _DT_WIDE[logits.dtype]
+    check(lib().cottus_sample_tokens(C.byref(p), _stream(stream)))
+    return (out, logprobs) if return_logprobs else out
 
 
 def paged_gather(kv_pool, block_table, context_lens, *, max_context, num_kv_heads, head_dim, block_size,

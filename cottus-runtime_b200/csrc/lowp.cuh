@@ -1,0 +1,136 @@
+// Building blocks of the norm, 8-bit and sampling kernels: bf16 and e4m3
+// conversions, group scales, host-side argument checks.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <string>
+
+#include "common.cuh"
+#include "cottus_b200.h"
+
+namespace cb200 {
+
+int set_error(int code, const std::string& msg);
+
+constexpr float kE4m3Max = 448.f;           // largest finite e4m3 value
+constexpr float kMinScale = 1.17549435e-38f;  // 2^-126: the scale of an all-zero group
+
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+__device__ __forceinline__ uint32_t pack_bf2(float a, float b) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7]));
+}
+
+// Eight consecutive elements that this kernel reads once (no L1 allocation;
+// a plain coherent load, so the buffer may be the kernel's output as well).
+__device__ __forceinline__ uint4 ld_once(const void* p) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(p));
+    return r;
+}
+__device__ __forceinline__ void load8_stream(const float* p, float (&v)[8]) {
+    const uint4 a = ld_once(p), b = ld_once(p + 4);
+    v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+    v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
+}
+__device__ __forceinline__ void load8_stream(const __half* p, float (&v)[8]) {
+    const uint4 r = ld_once(p);
+    const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = h2_to_f2(u[i]);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void load8_stream(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 r = ld_once(p);
+    const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // a bf16 is the upper half of an fp32
+        v[2 * i] = __uint_as_float(u[i] << 16);
+        v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    }
+}
+
+// Maximum that keeps a NaN of either side.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float amax8(const float (&v)[8]) {
+    float m = fabsf(v[0]);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
+    return m;
+}
+// Maximum over each half of the warp (all 32 lanes take part).
+__device__ __forceinline__ float amax16(float m) {
+#pragma unroll
+    for (int o = 8; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
+__device__ __forceinline__ float group_scale(float amax) { return max_nan(__fdiv_rn(amax, kE4m3Max), kMinScale); }
+
+// value / scale in e4m3, to nearest even, magnitudes above 448 to 448, NaN kept.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float s) {
+    uint2 r;
+    r.x = e4m3x2(__fdiv_rn(v[0], s), __fdiv_rn(v[1], s)) | (e4m3x2(__fdiv_rn(v[2], s), __fdiv_rn(v[3], s)) << 16);
+    r.y = e4m3x2(__fdiv_rn(v[4], s), __fdiv_rn(v[5], s)) | (e4m3x2(__fdiv_rn(v[6], s), __fdiv_rn(v[7], s)) << 16);
+    return r;
+}
+__device__ __forceinline__ uint8_t e4m3(float v, float s) { return (uint8_t)(e4m3x2(__fdiv_rn(v, s), 0.f) & 0xFFu); }
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+inline bool lowp_input_dtype(int32_t t) { return t == COTTUS_F32 || t == COTTUS_F16 || t == COTTUS_BF16; }
+inline int dtype_bytes(int32_t t) { return t == COTTUS_F32 ? 4 : (t == COTTUS_E4M3 ? 1 : 2); }
+inline bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+struct Span {
+    const void* p;
+    size_t bytes;
+};
+inline bool overlap(const Span& a, const Span& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+}
+
+// Launch that may start while the stream's preceding kernel drains: the
+// kernel calls grid_dependency_wait() before it touches global memory, and
+// only then grid_dependents_launch(), so that whatever follows starts after
+// everything before this kernel is complete.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                              Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+}  // namespace cb200

@@ -1,0 +1,400 @@
+// RMS norm with the residual's addition, and quantisation to e4m3 with one
+// scale per 128 values.  Replaces residualAddCUDA + rmsnormCUDA
+// (compute_primitives_cuda.cu:58-89), whose every thread sums the whole row.
+//
+//   h = x (+ r);  y = h * (mean(h^2) + eps)^(-1/2) * g
+//   s = max(amax_128 |y| / 448, 2^-126);  q = e4m3(y / s)
+//
+// Both only move bytes (a few operations per element), so HBM bounds them at
+// many rows and the latency of one load, one block reduction and one store at
+// few.  Each input is read once: a row stays in registers between the sum of
+// squares and the output.  Eight consecutive elements per thread and step
+// (16 bytes of a 16-bit type), so that 16 neighbouring lanes hold one group
+// of 128 and its amax is four shuffles.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <string>
+
+#include "common.cuh"
+#include "cottus_b200.h"
+#include "internal.h"
+#include "lowp.cuh"
+
+namespace cb200 {
+
+namespace {
+
+struct NormArgs {
+    const void* x;
+    const float* residual;
+    float* residual_out;
+    const float* weight;
+    void* out;
+    float* scales;
+    long long rows;
+    int hidden, out_dtype;
+    float eps;
+};
+
+// Sum over the block, the same value in every thread (fixed order).
+__device__ __forceinline__ float block_sum(float v, float* smem) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (lane == 0) smem[warp] = v;
+    __syncthreads();
+    v = lane < warps ? smem[lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+__device__ __forceinline__ void store_out8(void* out, int dtype, size_t e, const float (&y)[8]) {
+    if (dtype == COTTUS_F32) store8(reinterpret_cast<float*>(out) + e, y);
+    else if (dtype == COTTUS_F16) store8(reinterpret_cast<__half*>(out) + e, y);
+    else store8(reinterpret_cast<__nv_bfloat16*>(out) + e, y);
+}
+__device__ __forceinline__ void store_out1(void* out, int dtype, size_t e, float y) {
+    if (dtype == COTTUS_F32) reinterpret_cast<float*>(out)[e] = y;
+    else if (dtype == COTTUS_F16) reinterpret_cast<__half*>(out)[e] = __float2half_rn(y);
+    else reinterpret_cast<__nv_bfloat16*>(out)[e] = __float2bfloat16_rn(y);
+}
+
+// One CTA per row, the row in registers: thread t holds the vectors of eight
+// t, t + T, ... (V of them).  hidden a multiple of 8, all rows 16-byte aligned.
+template <typename XT, int V>
+__global__ void rms_norm_vec_kernel(const NormArgs a) {
+    __shared__ float red[32];
+    const int nvec = a.hidden >> 3, T = blockDim.x;
+    const long long row = blockIdx.x;
+    const XT* x = reinterpret_cast<const XT*>(a.x) + row * a.hidden;
+    grid_dependency_wait();
+    grid_dependents_launch();
+    float h[V][8];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int v = threadIdx.x + i * T;
+        if (v < nvec) load8_stream(x + v * 8, h[i]);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[i][j] = 0.f;
+    }
+    if (a.residual) {
+        const float* r = a.residual + row * a.hidden;
+        float* ro = a.residual_out + row * a.hidden;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int v = threadIdx.x + i * T;
+            if (v < nvec) {
+                float t[8];
+                load8_stream(r + v * 8, t);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[i][j] += t[j];
+                store8(ro + v * 8, h[i]);
+            }
+        }
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = fmaf(h[i][j], h[i][j], ss);
+    ss = block_sum(ss, red);
+    const float inv = __frsqrt_rn(__fdiv_rn(ss, (float)a.hidden) + a.eps);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int v = threadIdx.x + i * T;
+        const bool live = v < nvec;
+        float w[8];
+        if (live) load8(a.weight + v * 8, w);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[i][j] = live ? h[i][j] * inv * w[j] : 0.f;
+        const size_t e = (size_t)row * a.hidden + v * 8;
+        if (a.out_dtype != COTTUS_E4M3) {
+            if (live) store_out8(a.out, a.out_dtype, e, h[i]);
+            continue;
+        }
+        const float s = group_scale(amax16(amax8(h[i])));
+        if (live) {
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.out) + e) = e4m3x8(h[i], s);
+            if ((v & 15) == 0) a.scales[(size_t)(v >> 4) * a.rows + row] = s;
+        }
+    }
+}
+
+// Any width and alignment: one CTA per row, the row read twice (the second
+// time from L1 or L2), one warp per group of 128.
+template <typename XT>
+__global__ void __launch_bounds__(512) rms_norm_any_kernel(const NormArgs a) {
+    __shared__ float red[32];
+    const long long row = blockIdx.x;
+    const size_t base = (size_t)row * a.hidden;
+    const XT* x = reinterpret_cast<const XT*>(a.x) + base;
+    grid_dependency_wait();
+    grid_dependents_launch();
+    float ss = 0.f;
+    for (int i = threadIdx.x; i < a.hidden; i += blockDim.x) {
+        float h = to_f32(x[i]);
+        if (a.residual) h += a.residual[base + i];
+        ss = fmaf(h, h, ss);
+    }
+    ss = block_sum(ss, red);  // (its barrier: every read of the row above precedes every write below)
+    const float inv = __frsqrt_rn(__fdiv_rn(ss, (float)a.hidden) + a.eps);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int groups = (a.hidden + 127) / 128;
+    for (int g = warp; g < groups; g += warps) {
+        float y[4];
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = g * 128 + j * 32 + lane;
+            y[j] = 0.f;
+            if (i < a.hidden) {
+                float h = to_f32(x[i]);
+                if (a.residual) {
+                    h += a.residual[base + i];
+                    a.residual_out[base + i] = h;
+                }
+                y[j] = h * inv * a.weight[i];
+                if (a.out_dtype != COTTUS_E4M3) store_out1(a.out, a.out_dtype, base + i, y[j]);
+            }
+            m = max_nan(m, fabsf(y[j]));
+        }
+        if (a.out_dtype == COTTUS_E4M3) {
+            const float s = group_scale(max_nan(amax16(m), __shfl_xor_sync(0xffffffffu, amax16(m), 16)));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = g * 128 + j * 32 + lane;
+                if (i < a.hidden) reinterpret_cast<uint8_t*>(a.out)[base + i] = e4m3(y[j], s);
+            }
+            if (lane == 0) a.scales[(size_t)g * a.rows + row] = s;
+        }
+    }
+}
+
+template <typename XT>
+cudaError_t launch_norm(const NormArgs& a, bool vec, cudaStream_t st) {
+    // one row per CTA; the grid's x dimension holds any row count below 2^31
+    if (!vec) {
+        const int want = (a.hidden + 31) / 32 * 32;
+        return launch_pdl(rms_norm_any_kernel<XT>, dim3((unsigned)a.rows), dim3(want < 512 ? want : 512), 0, st, a);
+    }
+    const int nvec = a.hidden / 8;
+    auto threads = [&](int V) { return ((nvec + V - 1) / V + 31) / 32 * 32; };
+    const dim3 grid((unsigned)a.rows);
+    if (nvec <= 512) return launch_pdl(rms_norm_vec_kernel<XT, 1>, grid, dim3(threads(1)), 0, st, a);
+    if (nvec <= 1024) return launch_pdl(rms_norm_vec_kernel<XT, 2>, grid, dim3(threads(2)), 0, st, a);
+    return launch_pdl(rms_norm_vec_kernel<XT, 4>, grid, dim3(threads(4)), 0, st, a);
+}
+
+// ---------------------------------------------------------------------------
+// quantisation
+// ---------------------------------------------------------------------------
+struct QuantArgs {
+    const void* x;
+    uint8_t* out;
+    float* scales;
+    long long rows;
+    int cols;
+};
+
+// Rows: half a warp per (row, group of 128).  VEC: eight elements per lane
+// (cols a multiple of 8, x 16-byte and out 8-byte aligned); else lanes take
+// every 16th element.
+template <typename XT, bool VEC>
+__global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
+    const int groups = (a.cols + 127) / 128;
+    const long long total = a.rows * groups;
+    const long long id = (blockIdx.x * (long long)blockDim.x + threadIdx.x) >> 4;
+    const int lane = threadIdx.x & 15;
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const bool live = id < total;
+    const long long row = live ? id / groups : 0;
+    const int g = live ? (int)(id - row * groups) : 0;
+    const size_t base = (size_t)row * a.cols + (size_t)g * 128;
+    const int n = live ? (a.cols - g * 128 < 128 ? a.cols - g * 128 : 128) : 0;
+    const XT* x = reinterpret_cast<const XT*>(a.x) + base;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    if constexpr (VEC) {
+        if (lane * 8 < n) load8_stream(x + lane * 8, v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (lane + j * 16 < n) v[j] = to_f32(x[lane + j * 16]);
+    }
+    const float s = group_scale(amax16(amax8(v)));
+    if constexpr (VEC) {
+        if (lane * 8 < n) *reinterpret_cast<uint2*>(a.out + base + lane * 8) = e4m3x8(v, s);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (lane + j * 16 < n) a.out[base + lane + j * 16] = e4m3(v[j], s);
+    }
+    if (live && lane == 0) a.scales[(size_t)g * a.rows + row] = s;
+}
+
+// Blocks: one CTA per 128 x 128 block, 64 elements per thread in registers.
+template <typename XT, bool VEC>
+__global__ void __launch_bounds__(256) quant_blocks_kernel(const QuantArgs a) {
+    __shared__ float red[8];
+    const int cb = blockIdx.x, groups = gridDim.x;
+    const long long rb = blockIdx.y;
+    const int c0 = cb * 128;
+    const int nc = a.cols - c0 < 128 ? a.cols - c0 : 128;
+    const int lane = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+    grid_dependency_wait();
+    grid_dependents_launch();
+    float v[8][8];
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const long long row = rb * 128 + r0 + i * 16;
+        const XT* x = reinterpret_cast<const XT*>(a.x) + (size_t)row * a.cols + c0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+        if (row < a.rows) {
+            if constexpr (VEC) {
+                if (lane * 8 < nc) load8_stream(x + lane * 8, v[i]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (lane + j * 16 < nc) v[i][j] = to_f32(x[lane + j * 16]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max_nan(m, amax8(v[i]));
+    m = amax16(m);
+    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 16));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = max_nan(m, red[w]);
+    const float s = group_scale(m);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const long long row = rb * 128 + r0 + i * 16;
+        if (row >= a.rows) continue;
+        uint8_t* o = a.out + (size_t)row * a.cols + c0;
+        if constexpr (VEC) {
+            if (lane * 8 < nc) *reinterpret_cast<uint2*>(o + lane * 8) = e4m3x8(v[i], s);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (lane + j * 16 < nc) o[lane + j * 16] = e4m3(v[i][j], s);
+        }
+    }
+    if (threadIdx.x == 0) a.scales[(size_t)rb * groups + cb] = s;
+}
+
+template <typename XT, bool VEC>
+cudaError_t launch_quant(const QuantArgs& a, bool blocks, cudaStream_t st) {
+    const long long groups = (a.cols + 127) / 128;
+    if (blocks)
+        return launch_pdl(quant_blocks_kernel<XT, VEC>, dim3((unsigned)groups, (unsigned)((a.rows + 127) / 128)),
+                          dim3(256), 0, st, a);
+    return launch_pdl(quant_rows_kernel<XT, VEC>, dim3((unsigned)((a.rows * groups + 15) / 16)), dim3(256), 0, st, a);
+}
+
+int fail(int code, const std::string& msg) { return set_error(code, msg); }
+int cuda_fail(cudaError_t e) { return fail(COTTUS_ERR_CUDA, std::string("CUDA error: ") + cudaGetErrorString(e)); }
+
+}  // namespace
+}  // namespace cb200
+
+extern "C" {
+
+int cottus_rms_norm(const cottus_rms_norm_params* p, cottus_stream_t stream) {
+    using namespace cb200;
+    if (!p) return fail(COTTUS_ERR_INVALID_ARGUMENT, "params must not be NULL");
+    if (p->rows < 0 || p->hidden <= 0) return fail(COTTUS_ERR_INVALID_ARGUMENT, "rows must be non-negative and hidden positive");
+    if (!lowp_input_dtype(p->x_dtype)) return fail(COTTUS_ERR_INVALID_ARGUMENT, "unknown x dtype");
+    if (!lowp_input_dtype(p->out_dtype) && p->out_dtype != COTTUS_E4M3)
+        return fail(COTTUS_ERR_INVALID_ARGUMENT, "unknown out dtype");
+    if (!(p->eps >= 0.f) || std::isinf(p->eps)) return fail(COTTUS_ERR_INVALID_ARGUMENT, "eps must be non-negative and finite");
+    if (p->rows == 0) return COTTUS_OK;
+    if (!p->x || !p->weight || !p->out) return fail(COTTUS_ERR_INVALID_ARGUMENT, "NULL pointer argument");
+    if (!p->residual != !p->residual_out)
+        return fail(COTTUS_ERR_INVALID_ARGUMENT, "give both residual and residual_out or neither");
+    if ((p->out_dtype == COTTUS_E4M3) != (p->scales != nullptr))
+        return fail(COTTUS_ERR_INVALID_ARGUMENT, "scales go with an e4m3 output, and only with one");
+    if (p->rows >= (int64_t(1) << 31)) return fail(COTTUS_ERR_UNSUPPORTED, "too many rows for one launch");
+    const size_t n = (size_t)p->rows * p->hidden;
+    const int xs = dtype_bytes(p->x_dtype), os = dtype_bytes(p->out_dtype);
+    const size_t sb = p->scales ? (size_t)p->rows * ((p->hidden + 127) / 128) * 4 : 0;
+    const Span sx{p->x, n * xs}, sr{p->residual, p->residual ? n * 4 : 0}, sro{p->residual_out, p->residual ? n * 4 : 0},
+        sw{p->weight, (size_t)p->hidden * 4}, so{p->out, n * os}, ss{p->scales, sb};
+    if ((overlap(so, sx) && !(p->out == p->x && os == xs)) || overlap(so, sr) || overlap(so, sro) || overlap(so, sw) ||
+        overlap(so, ss) || (overlap(sro, sr) && p->residual_out != p->residual) || overlap(sro, sx) ||
+        overlap(sro, sw) || overlap(ss, sx) || overlap(ss, sr) || overlap(ss, sro) || overlap(ss, sw))
+        return fail(COTTUS_ERR_INVALID_ARGUMENT, "an output overlaps another buffer");
+    if (!aligned(p->x, xs) || !aligned(p->out, os) || !aligned(p->residual, 4) || !aligned(p->residual_out, 4) ||
+        !aligned(p->weight, 4) || !aligned(p->scales, 4))
+        return fail(COTTUS_ERR_INVALID_ARGUMENT, "a pointer is not aligned to its element");
+    NormArgs a;
+    a.x = p->x;
+    a.residual = p->residual;
+    a.residual_out = p->residual_out;
+    a.weight = p->weight;
+    a.out = p->out;
+    a.scales = p->scales;
+    a.rows = p->rows;
+    a.hidden = p->hidden;
+    a.out_dtype = p->out_dtype;
+    a.eps = p->eps;
+    // the register kernel holds rows of up to 32768 elements (4 vectors of 8 per thread)
+    const bool vec = p->hidden % 8 == 0 && p->hidden <= 32768 && aligned(p->x, 16) && aligned(p->residual, 16) &&
+                     aligned(p->residual_out, 16) && aligned(p->weight, 16) && aligned(p->out, os == 1 ? 8 : 16);
+    const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const cudaError_t e = p->x_dtype == COTTUS_F32   ? launch_norm<float>(a, vec, st)
+                          : p->x_dtype == COTTUS_F16 ? launch_norm<__half>(a, vec, st)
+                                                     : launch_norm<__nv_bfloat16>(a, vec, st);
+    return e == cudaSuccess ? COTTUS_OK : cuda_fail(e);
+}
+
+int cottus_quantize_fp8(const cottus_quantize_params* p, cottus_stream_t stream) {
+    using namespace cb200;
+    if (!p) return fail(COTTUS_ERR_INVALID_ARGUMENT, "params must not be NULL");
+    if (p->rows < 0 || p->cols <= 0) return fail(COTTUS_ERR_INVALID_ARGUMENT, "rows must be non-negative and cols positive");
+    if (!lowp_input_dtype(p->x_dtype)) return fail(COTTUS_ERR_INVALID_ARGUMENT, "unknown x dtype");
+    if (p->block_rows != 1 && p->block_rows != 128) return fail(COTTUS_ERR_INVALID_ARGUMENT, "block_rows must be 1 or 128");
+    if (p->rows == 0) return COTTUS_OK;
+    if (!p->x || !p->out || !p->scales) return fail(COTTUS_ERR_INVALID_ARGUMENT, "NULL pointer argument");
+    const bool blocks = p->block_rows == 128;
+    const int64_t groups = (p->cols + 127) / 128, row_blocks = (p->rows + 127) / 128;
+    if (blocks ? row_blocks > 65535 : p->rows >= (int64_t(1) << 35) / groups)
+        return fail(COTTUS_ERR_UNSUPPORTED, "too many rows for one launch");
+    const size_t n = (size_t)p->rows * p->cols;
+    const int xs = dtype_bytes(p->x_dtype);
+    const Span sx{p->x, n * xs}, so{p->out, n}, ss{p->scales, (size_t)((blocks ? row_blocks : p->rows) * groups) * 4};
+    if (overlap(so, sx) || overlap(so, ss) || overlap(ss, sx))
+        return fail(COTTUS_ERR_INVALID_ARGUMENT, "an output overlaps another buffer");
+    if (!aligned(p->x, xs) || !aligned(p->scales, 4))
+        return fail(COTTUS_ERR_INVALID_ARGUMENT, "a pointer is not aligned to its element");
+    QuantArgs a;
+    a.x = p->x;
+    a.out = static_cast<uint8_t*>(p->out);
+    a.scales = p->scales;
+    a.rows = p->rows;
+    a.cols = p->cols;
+    const bool vec = p->cols % 8 == 0 && aligned(p->x, 16) && aligned(p->out, 8);
+    const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    auto run = [&](auto zero) {
+        using XT = decltype(zero);
+        return vec ? launch_quant<XT, true>(a, blocks, st) : launch_quant<XT, false>(a, blocks, st);
+    };
+    const cudaError_t e = p->x_dtype == COTTUS_F32   ? run(float{})
+                          : p->x_dtype == COTTUS_F16 ? run(__half{})
+                                                     : run(__nv_bfloat16{});
+    return e == cudaSuccess ? COTTUS_OK : cuda_fail(e);
+}
+
+}  // extern "C"

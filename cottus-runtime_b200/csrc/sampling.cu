@@ -1,0 +1,695 @@
+// One token per row of logits: temperature, top-k, top-p and min-p, drawn
+// with a given uniform number.  Replaces the device-to-host copy of the
+// logits and the host argmax (engine.cpp:85-87).
+//
+// With the candidates ordered by (logit descending, index ascending) every
+// filter keeps a prefix, so the kept set is { order key <= threshold } (and,
+// for min-p, weight >= min_p, which is a prefix as well).  The order key of a
+// logit is the 64-bit integer (descending image of its fp32 bits, index): all
+// keys of a row differ, so ties need no special case.
+//
+// A row belongs to one thread-block cluster; each CTA holds a contiguous
+// slice of it in shared memory and the row is read from HBM once.
+//   1. smallest key (= the maximum, at its lowest index);
+//   2. with top-k or top-p: a histogram (count, mass) of the distance to the
+//      maximum, 128 bins per octave, merged over the cluster; the bin in
+//      which the count or the mass passes its target; its few members are
+//      gathered by the first CTA, sorted by key, and the threshold is read
+//      off their prefix sums.  A bin with more members than the list holds is
+//      first split by histograms of the key itself;
+//   3. the kept mass per warp, each warp owning a contiguous run of indices,
+//      then the one warp whose run holds uniform * mass walks it.
+//
+// Weights: exp in fp64, held as 64-bit fixed point (47 - 43 fractional bits,
+// so that a row's sum fits).  Integer sums do not depend on their order, so
+// atomics leave no trace in the result, and a border is missed only where the
+// draw falls within 2^-45 or so of it.
+//
+// Bounds: HBM for many rows; at one row the chain of cluster barriers (about
+// nine with all filters).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <string>
+
+#include "common.cuh"
+#include "cottus_b200.h"
+#include "internal.h"
+#include "lowp.cuh"
+
+namespace cb200 {
+int device_sm_count(int device);
+
+namespace {
+
+using u64 = unsigned long long;
+
+constexpr int kT = 512;        // threads per CTA
+constexpr int kW = kT / 32;
+constexpr int kBins = 1024;    // 8 octaves of distance to the maximum, 0.25 to 64
+constexpr int kList = 2048;    // members of a bin that are sorted directly
+constexpr int kMaxCluster = 8; // portable cluster size
+constexpr u64 kNoKey = ~0ull;
+
+struct SampleArgs {
+    const void* logits;
+    const float* uniforms;
+    const float* temperature;
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    int32_t* tokens;
+    float* logprobs;
+    uint32_t* status;
+    int vocab, slice, raw_bytes, frac_bits;
+};
+
+// Shared memory behind the slice.
+struct Shared {
+    union {
+        uint32_t hist[4][kBins];  // count and three 16-bit limbs of the mass
+        u64 list[kList];
+    };
+    uint32_t mcnt[kBins];  // merged over the cluster
+    u64 mmass[kBins];
+    u64 wsum[kW];
+    uint32_t wcnt[kW];
+    u64 slot[2][kMaxCluster];  // one word from each CTA
+    u64 res[4];                // broadcast by the first CTA
+    u64 pick_mass;
+    uint32_t pick_cnt, pick_bin, list_n;
+};
+
+__device__ __forceinline__ void carrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cwait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void csync() {
+    carrive();
+    cwait();
+}
+__device__ __forceinline__ uint32_t mapa(const void* local, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(local)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void st_cluster(uint32_t a, u64 v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t a, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_cluster(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t atom_add_cluster(uint32_t a, uint32_t v) {
+    uint32_t r;
+    asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(r) : "r"(a), "r"(v) : "memory");
+    return r;
+}
+
+__device__ __forceinline__ u64 shfl_xor(u64 v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
+__device__ __forceinline__ u64 warp_sum(u64 v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += shfl_xor(v, o);
+    return v;
+}
+__device__ __forceinline__ u64 warp_min(u64 v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const u64 w = shfl_xor(v, o);
+        v = w < v ? w : v;
+    }
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ T warp_scan(T v, int lane) {  // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const T w = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += w;
+    }
+    return v;
+}
+
+// fp32 -> 32 bits whose unsigned order is descending value (-0 as +0), and back.
+__device__ __forceinline__ uint32_t desc_bits(float x) {
+    const uint32_t b = __float_as_uint(x + 0.f);
+    return ~(b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u));
+}
+__device__ __forceinline__ float from_desc(uint32_t d) {
+    const uint32_t k = ~d;
+    return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+__device__ __forceinline__ bool candidate(float x) { return x > -INFINITY; }  // false for -inf and NaN
+__device__ __forceinline__ u64 order_key(float x, uint32_t index) { return ((u64)desc_bits(x) << 32) | index; }
+
+// The weight of a logit: exp in fp64, 0 where fixed point cannot hold it.
+struct Weight {
+    float top;
+    double inv_t, unit, least;
+    __device__ __forceinline__ double z(float x) const { return ((double)x - (double)top) * inv_t; }
+    __device__ __forceinline__ double operator()(float x) const {
+        if (x == top) return 1.0;
+        if (top == INFINITY) return 0.0;
+        const double v = z(x);
+        return v < least ? 0.0 : exp(v);
+    }
+    __device__ __forceinline__ u64 fixed(double w) const { return __double2ull_rn(w * unit); }
+};
+
+// Level-one bin: monotone in the distance to the maximum.
+__device__ __forceinline__ int distance_bin(float top, float x) {
+    if (x == top) return 0;
+    const int b = (int)(__float_as_uint(top - x) >> 16) - (125 << 7);
+    return b < 0 ? 0 : (b < kBins ? b : kBins - 1);
+}
+
+template <typename XT>
+struct Row {
+    const SampleArgs& a;
+    Shared& s;
+    const XT* x;    // the slice in shared memory
+    int lo, n;      // its first index and length
+    int rank, size; // of this CTA in the cluster
+    Weight weight;
+
+    __device__ __forceinline__ float at(int i) const { return to_f32(x[i]); }
+
+    __device__ void clear_hist() const {
+        for (int i = threadIdx.x; i < 4 * kBins; i += kT) s.hist[0][i] = 0;
+        __syncthreads();
+    }
+    __device__ __forceinline__ void add(int bin, float v, bool mass) const {
+        atomicAdd(&s.hist[0][bin], 1u);
+        if (mass) {
+            const u64 w = weight.fixed(weight(v));
+            if (w & 0xFFFF) atomicAdd(&s.hist[1][bin], (uint32_t)(w & 0xFFFF));
+            if ((w >> 16) & 0xFFFF) atomicAdd(&s.hist[2][bin], (uint32_t)((w >> 16) & 0xFFFF));
+            if (w >> 32) atomicAdd(&s.hist[3][bin], (uint32_t)(w >> 32));
+        }
+    }
+    // Merges the cluster's histograms into every CTA's mcnt / mmass.
+    __device__ void merge_hist() const {
+        csync();
+        const int per = kBins / size;
+        for (int i = threadIdx.x; i < per; i += kT) {
+            const int b = rank * per + i;
+            uint32_t c = 0;
+            u64 m = 0;
+            for (int q = 0; q < size; ++q) {
+                c += ld_cluster(mapa(&s.hist[0][b], q));
+                m += (u64)ld_cluster(mapa(&s.hist[1][b], q)) + ((u64)ld_cluster(mapa(&s.hist[2][b], q)) << 16) +
+                     ((u64)ld_cluster(mapa(&s.hist[3][b], q)) << 32);
+            }
+            for (int q = 0; q < size; ++q) {
+                st_cluster(mapa(&s.mcnt[b], q), c);
+                st_cluster(mapa(&s.mmass[b], q), m);
+            }
+        }
+        csync();
+    }
+
+    struct Pick {
+        int bin;  // kBins: none
+        uint32_t before_cnt, in_cnt;
+        u64 before_mass;
+    };
+    // The bin in which the running count reaches k (by_mass false) or the
+    // running mass, on top of mass0, reaches t.
+    __device__ Pick pick_bin(bool by_mass, uint32_t k, u64 mass0, double t) const {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        constexpr int PER = kBins / kT;
+        uint32_t c = 0;
+        u64 m = 0;
+        for (int j = 0; j < PER; ++j) {
+            c += s.mcnt[threadIdx.x * PER + j];
+            m += s.mmass[threadIdx.x * PER + j];
+        }
+        const uint32_t ci = warp_scan(c, lane);
+        const u64 mi = warp_scan(m, lane);
+        if (lane == 31) {
+            s.wcnt[warp] = ci;
+            s.wsum[warp] = mi;
+        }
+        if (threadIdx.x == 0) s.pick_bin = kBins;
+        __syncthreads();
+        uint32_t cb = ci - c;
+        u64 mb = mi - m;
+        for (int w = 0; w < warp; ++w) {
+            cb += s.wcnt[w];
+            mb += s.wsum[w];
+        }
+        for (int j = 0; j < PER; ++j) {
+            const int b = threadIdx.x * PER + j;
+            const uint32_t cc = s.mcnt[b];
+            const u64 mm = s.mmass[b];
+            const bool before = by_mass ? (double)(mass0 + mb) < t || (mass0 + mb == 0) : cb < k;
+            const bool reached = by_mass ? (double)(mass0 + mb + mm) >= t : cb + cc >= k;
+            // the first bin that reaches the target from below is the pick
+            // (empty bins before it reach nothing new)
+            if (cc && before && reached) atomicMin(&s.pick_bin, (uint32_t)b);
+            cb += cc;
+            mb += mm;
+        }
+        __syncthreads();
+        const int bin = (int)s.pick_bin;
+        // sums before the picked bin, by its owner
+        if (bin < kBins && threadIdx.x == bin / PER) {
+            uint32_t c2 = ci - c;
+            u64 m2 = mi - m;
+            for (int w = 0; w < warp; ++w) {
+                c2 += s.wcnt[w];
+                m2 += s.wsum[w];
+            }
+            for (int j = threadIdx.x * PER; j < bin; ++j) {
+                c2 += s.mcnt[j];
+                m2 += s.mmass[j];
+            }
+            s.pick_cnt = c2;
+            s.pick_mass = m2;
+        }
+        __syncthreads();
+        Pick p;
+        p.bin = bin;
+        p.before_cnt = bin < kBins ? s.pick_cnt : 0;
+        p.before_mass = bin < kBins ? s.pick_mass : 0;
+        p.in_cnt = bin < kBins ? s.mcnt[bin] : 0;
+        __syncthreads();
+        return p;
+    }
+
+    // Level one: the histogram of the distance to the maximum.
+    __device__ void build_l1(bool mass) const {
+        clear_hist();
+        for (int i = threadIdx.x; i < n; i += kT) {
+            const float v = at(i);
+            if (candidate(v)) add(distance_bin(weight.top, v), v, mass);
+        }
+        merge_hist();
+    }
+    // The mass of all candidates, from the level-one histogram.
+    __device__ u64 l1_mass() const {
+        u64 m = 0;
+        for (int b = threadIdx.x; b < kBins; b += kT) m += s.mmass[b];
+        m = warp_sum(m);
+        if ((threadIdx.x & 31) == 0) s.wsum[threadIdx.x >> 5] = m;
+        __syncthreads();
+        m = 0;
+        for (int w = 0; w < kW; ++w) m += s.wsum[w];
+        __syncthreads();
+        return m;
+    }
+
+    // The threshold key at which the running count reaches k, or the running
+    // mass reaches t, among the keys up to `limit`; `limit` where it does not.
+    // l1: the merged arrays hold the level-one histogram (with masses, where
+    // need_mass); false on return if they no longer do.  mass_to (need_mass):
+    // the mass of everything up to the threshold.
+    __device__ u64 select(bool by_mass, uint32_t k, double t, u64 limit, bool need_mass, bool& l1, u64& mass_to) const {
+        if (!l1) build_l1(need_mass);
+        l1 = true;
+        Pick p = pick_bin(by_mass, k, 0, t);
+        if (p.bin == kBins) {  // fewer candidates than k
+            mass_to = need_mass ? l1_mass() : 0;
+            return limit;
+        }
+        const int level_bin = p.bin;
+        u64 kmin = 0, kmax = limit;  // members: keys in this range (and, at first, of the picked bin)
+        bool by_bin = true;
+        uint32_t before_cnt = p.before_cnt;
+        u64 before_mass = p.before_mass;
+        auto member = [&](float v, u64 key) {
+            return by_bin ? distance_bin(weight.top, v) == level_bin && key <= limit : key >= kmin && key <= kmax;
+        };
+        while (p.in_cnt > (uint32_t)kList) {
+            // split the bin: its members' key range in kBins equal parts
+            u64 mn = kNoKey, mx = 0;
+            for (int i = threadIdx.x; i < n; i += kT) {
+                const float v = at(i);
+                if (!candidate(v)) continue;
+                const u64 key = order_key(v, (uint32_t)(lo + i));
+                if (!member(v, key)) continue;
+                mn = key < mn ? key : mn;
+                mx = key > mx ? key : mx;
+            }
+            mn = cluster_min(mn);
+            mx = ~cluster_min(~mx);
+            int sh = 0;
+            while (((mx - mn) >> sh) >= (u64)kBins) ++sh;
+            clear_hist();
+            for (int i = threadIdx.x; i < n; i += kT) {
+                const float v = at(i);
+                if (!candidate(v)) continue;
+                const u64 key = order_key(v, (uint32_t)(lo + i));
+                if (member(v, key)) add((int)((key - mn) >> sh), v, need_mass);
+            }
+            merge_hist();
+            l1 = false;
+            p = pick_bin(by_mass, k - before_cnt, before_mass, t);
+            before_cnt += p.before_cnt;
+            before_mass += p.before_mass;
+            by_bin = false;
+            kmin = mn + ((u64)p.bin << sh);
+            kmax = kmin + (((u64)1 << sh) - 1);
+            if (kmax > mx) kmax = mx;
+        }
+        // gather the members in the first CTA
+        if (threadIdx.x == 0) s.list_n = 0;
+        csync();  // (also: nobody reads a histogram any more, the list may take its place)
+        {
+            const int lane = threadIdx.x & 31;
+            const uint32_t counter = mapa(&s.list_n, 0), list0 = mapa(&s.list[0], 0);
+            for (int i0 = threadIdx.x - lane; i0 < n; i0 += kT) {
+                const int i = i0 + lane;
+                const float v = i < n ? at(i) : -INFINITY;
+                const u64 key = order_key(v, (uint32_t)(lo + i));
+                const bool in = candidate(v) && member(v, key);
+                const uint32_t mask = __ballot_sync(0xffffffffu, in);
+                if (!mask) continue;
+                uint32_t at0 = 0;
+                if (lane == 0) at0 = atom_add_cluster(counter, __popc(mask));
+                at0 = __shfl_sync(0xffffffffu, at0, 0);
+                const uint32_t pos = at0 + __popc(mask & ((1u << lane) - 1));
+                if (in && pos < (uint32_t)kList) st_cluster(list0 + pos * 8, key);
+            }
+        }
+        csync();
+        if (rank == 0) {
+            const int m = (int)(s.list_n < (uint32_t)kList ? s.list_n : (uint32_t)kList);
+            int pow2 = 2;
+            while (pow2 < m) pow2 <<= 1;
+            for (int i = m + threadIdx.x; i < pow2; i += kT) s.list[i] = kNoKey;
+            __syncthreads();
+            for (int w = 2; w <= pow2; w <<= 1)
+                for (int j = w >> 1; j; j >>= 1) {
+                    for (int i = threadIdx.x; i < pow2 / 2; i += kT) {
+                        const int p0 = ((i & ~(j - 1)) << 1) | (i & (j - 1)), p1 = p0 | j;
+                        const u64 u = s.list[p0], v = s.list[p1];
+                        if ((u > v) == ((p0 & w) == 0)) {
+                            s.list[p0] = v;
+                            s.list[p1] = u;
+                        }
+                    }
+                    __syncthreads();
+                }
+            // prefix masses of the sorted members, in runs of `per` per thread
+            const int per = (m + kT - 1) / kT;
+            const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+            u64 own = 0;
+            if (need_mass)
+                for (int j = 0; j < per; ++j) {
+                    const int i = threadIdx.x * per + j;
+                    if (i < m) own += weight.fixed(weight(from_desc((uint32_t)(s.list[i] >> 32))));
+                }
+            const u64 incl = warp_scan(own, lane);
+            if (lane == 31) s.wsum[warp] = incl;
+            if (threadIdx.x == 0) s.pick_bin = 0x7fffffffu;
+            __syncthreads();
+            u64 run = before_mass + incl - own;
+            for (int w = 0; w < warp; ++w) run += s.wsum[w];
+            const u64 run0 = run;
+            for (int j = 0; j < per; ++j) {
+                const int i = threadIdx.x * per + j;
+                if (i >= m) break;
+                if (need_mass) run += weight.fixed(weight(from_desc((uint32_t)(s.list[i] >> 32))));
+                const bool hit = i == m - 1 || (by_mass ? (double)run >= t : before_cnt + (uint32_t)i + 1 >= k);
+                if (hit) {
+                    atomicMin(&s.pick_bin, (uint32_t)i);
+                    break;
+                }
+            }
+            __syncthreads();
+            const int hit = (int)s.pick_bin;
+            if (m == 0) {  // (a picked bin has members)
+                if (threadIdx.x < size) {
+                    st_cluster(mapa(&s.res[0], threadIdx.x), limit);
+                    st_cluster(mapa(&s.res[1], threadIdx.x), before_mass);
+                }
+            } else if (threadIdx.x == hit / per) {
+                u64 r = run0;
+                if (need_mass)
+                    for (int i = threadIdx.x * per; i <= hit; ++i)
+                        r += weight.fixed(weight(from_desc((uint32_t)(s.list[i] >> 32))));
+                const u64 key = s.list[hit];
+                for (int q = 0; q < size; ++q) {
+                    st_cluster(mapa(&s.res[0], q), key);
+                    st_cluster(mapa(&s.res[1], q), r);
+                }
+            }
+        }
+        csync();
+        mass_to = s.res[1];
+        const u64 thr = s.res[0];
+        __syncthreads();
+        return thr;
+    }
+
+    // Smallest v of the cluster's threads, in every thread.
+    __device__ u64 cluster_min(u64 v) const {
+        v = warp_min(v);
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        if (lane == 0) s.wsum[warp] = v;
+        __syncthreads();
+        if (warp == 0) {
+            v = warp_min(lane < kW ? s.wsum[lane] : kNoKey);
+            if (lane < size) st_cluster(mapa(&s.slot[0][rank], lane), v);
+        }
+        csync();
+        v = kNoKey;
+        for (int q = 0; q < size; ++q) v = s.slot[0][q] < v ? s.slot[0][q] : v;
+        csync();  // the slots may be written again
+        return v;
+    }
+};
+
+template <typename XT>
+__global__ void __launch_bounds__(kT) sample_kernel(const SampleArgs a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    Shared& s = *reinterpret_cast<Shared*>(smem + a.raw_bytes);
+    uint32_t rank_u, size_u;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank_u));
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size_u));
+    const int rank = (int)rank_u, size = (int)size_u;
+    const int row = blockIdx.x / size;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lo = rank * a.slice < a.vocab ? rank * a.slice : a.vocab;
+    const int n = a.vocab - lo < a.slice ? a.vocab - lo : a.slice;
+    const XT* g = reinterpret_cast<const XT*>(a.logits) + (size_t)row * a.vocab + lo;
+    const int mis = (int)(reinterpret_cast<uintptr_t>(g) & 15);
+    XT* x = reinterpret_cast<XT*>(smem + mis);
+    carrive();  // (awaited below: no CTA's shared memory is written before it has started)
+    grid_dependency_wait();
+    grid_dependents_launch();
+    // the slice, at the same offset from a 16-byte boundary as in memory:
+    // whole 16-byte runs, and single elements at its two ends
+    {
+        constexpr int E = 16 / (int)sizeof(XT);
+        const int head = mis ? ((16 - mis) / (int)sizeof(XT) < n ? (16 - mis) / (int)sizeof(XT) : n) : 0;
+        const int runs = (n - head) / E;
+        const uint4* src = reinterpret_cast<const uint4*>(g + head);
+        uint4* dst = reinterpret_cast<uint4*>(x + head);
+#pragma unroll 4
+        for (int i = threadIdx.x; i < runs; i += kT) dst[i] = ld_once(src + i);
+        if (threadIdx.x < head) x[threadIdx.x] = g[threadIdx.x];
+        const int tail = head + runs * E;
+        if (threadIdx.x < n - tail) x[tail + threadIdx.x] = g[tail + threadIdx.x];
+    }
+    float temp = a.temperature ? a.temperature[row] : 1.f;
+    const float u_in = a.uniforms[row];
+    int top_k = a.top_k ? a.top_k[row] : 0;
+    const float top_p = a.top_p ? a.top_p[row] : 1.f;
+    const float min_p = a.min_p ? a.min_p[row] : 0.f;
+    cwait();
+    __syncthreads();
+
+    Row<XT> r{a, s, x, lo, n, rank, size, {}};
+    u64 front = kNoKey;
+    for (int i = threadIdx.x; i < n; i += kT) {
+        const float v = r.at(i);
+        if (candidate(v)) {
+            const u64 key = order_key(v, (uint32_t)(lo + i));
+            front = key < front ? key : front;
+        }
+    }
+    front = r.cluster_min(front);
+    if (front == kNoKey || !(temp > 0.f)) {  // nothing to choose from, or greedy
+        if (rank == 0 && threadIdx.x == 0) {
+            const bool none = front == kNoKey;
+            a.tokens[row] = none ? -1 : (int32_t)(uint32_t)front;
+            if (a.logprobs) a.logprobs[row] = none ? -INFINITY : 0.f;
+            if (none) report(a.status, COTTUS_STATUS_NO_TOKEN);
+        }
+        return;
+    }
+    r.weight.top = from_desc((uint32_t)(front >> 32));
+    r.weight.inv_t = 1.0 / (double)temp;
+    r.weight.unit = (double)(1ull << a.frac_bits);
+    r.weight.least = -(a.frac_bits + 2) * 0.6931471805599453;
+
+    u64 thr = kNoKey;
+    const bool by_p = top_p < 1.f;  // (false for NaN)
+    const bool by_k = top_k > 0 && top_k < a.vocab;
+    bool l1 = false;
+    if (by_k) {
+        u64 mass = 0;
+        thr = r.select(false, (uint32_t)top_k, 0.0, kNoKey, by_p, l1, mass);
+        if (by_p) {
+            const double t = (double)top_p * (double)mass;
+            thr = r.select(true, 0, t, thr, true, l1, mass);
+        }
+    } else if (by_p) {
+        // the whole mass first: one histogram serves both
+        r.build_l1(true);
+        l1 = true;
+        u64 mass = r.l1_mass();
+        thr = r.select(true, 0, (double)top_p * (double)mass, kNoKey, true, l1, mass);
+    }
+
+    // the kept mass: each warp owns a contiguous run of indices
+    const int run = (n + kT - 1) / kT * 32;
+    const int w0 = warp * run, w1 = w0 + run < n ? w0 + run : n;
+    const double least_w = min_p > 0.f ? (double)min_p : 0.0;  // (0 for NaN)
+    auto kept = [&](int i) -> u64 {
+        const float v = r.at(i);
+        if (!candidate(v)) return 0;
+        const u64 key = order_key(v, (uint32_t)(lo + i));
+        if (key > thr) return 0;
+        const double w = r.weight(v);
+        return w >= least_w || key == front ? r.weight.fixed(w) : 0;
+    };
+    u64 own = 0;
+    for (int i = w0 + lane; i < w1; i += 32) own += kept(i);
+    own = warp_sum(own);
+    if (lane == 0) s.wsum[warp] = own;
+    __syncthreads();
+    u64 cta = 0;
+    for (int w = 0; w < kW; ++w) cta += s.wsum[w];
+    if (threadIdx.x < size) st_cluster(mapa(&s.slot[1][rank], threadIdx.x), cta);
+    csync();
+    u64 base = 0, total = 0;
+    for (int q = 0; q < size; ++q) {
+        if (q < rank) base += s.slot[1][q];
+        total += s.slot[1][q];
+    }
+    for (int w = 0; w < warp; ++w) base += s.wsum[w];
+    // uniform in [0, 1): 1 - 2^-24 is the largest fp32 below 1 (NaN counts as 0)
+    const float u = u_in > 0.f ? fminf(u_in, 0.99999994f) : 0.f;
+    const double t = (double)u * (double)total;
+    // the warp in whose run the running sum first exceeds t
+    if ((double)(base + own) > t && !((double)base > t)) {
+        u64 before = base;
+        for (int i0 = w0; i0 < w1; i0 += 32) {
+            const int i = i0 + lane;
+            const u64 m = i < w1 ? kept(i) : 0;
+            const u64 sum = before + warp_scan(m, lane);
+            const uint32_t hit = __ballot_sync(0xffffffffu, (double)sum > t);
+            if (hit) {
+                if (lane == __ffs(hit) - 1) {
+                    a.tokens[row] = lo + i;
+                    if (a.logprobs) {
+                        const float v = r.at(i);
+                        const double z = v == r.weight.top ? 0.0 : r.weight.z(v);
+                        a.logprobs[row] = (float)(z - log((double)total / r.weight.unit));
+                    }
+                }
+                break;
+            }
+            before = __shfl_sync(0xffffffffu, sum, 31);
+        }
+    }
+}
+
+// Dynamic shared memory of a CTA that holds `slice` logits.
+size_t sample_smem(int slice, int es) { return ((size_t)slice * es + 31) / 16 * 16 + sizeof(Shared); }
+
+template <typename XT>
+cudaError_t launch_sample(SampleArgs a, int batch, int cluster, cudaStream_t st) {
+    static std::atomic<uint64_t> ready{0};  // a bit per device
+    auto kern = sample_kernel<XT>;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+    }
+    a.slice = (a.vocab + cluster - 1) / cluster;
+    const size_t smem = sample_smem(a.slice, sizeof(XT));
+    a.raw_bytes = (int)(smem - sizeof(Shared));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((long long)batch * cluster));
+    cfg.blockDim = dim3(kT);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+int fail(int code, const std::string& msg) { return set_error(code, msg); }
+
+}  // namespace
+}  // namespace cb200
+
+extern "C" int cottus_sample_tokens(const cottus_sample_params* p, cottus_stream_t stream) {
+    using namespace cb200;
+    if (!p) return fail(COTTUS_ERR_INVALID_ARGUMENT, "params must not be NULL");
+    if (p->batch < 0 || p->vocab <= 0) return fail(COTTUS_ERR_INVALID_ARGUMENT, "batch must be non-negative and vocab positive");
+    if (!lowp_input_dtype(p->dtype)) return fail(COTTUS_ERR_INVALID_ARGUMENT, "unknown dtype");
+    if (p->vocab > COTTUS_MAX_VOCAB)
+        return fail(COTTUS_ERR_UNSUPPORTED, "vocab must be at most " + std::to_string(COTTUS_MAX_VOCAB));
+    if (p->batch == 0) return COTTUS_OK;
+    if (p->batch > (1 << 27)) return fail(COTTUS_ERR_UNSUPPORTED, "too many rows for one launch");
+    if (!p->logits || !p->uniforms || !p->tokens) return fail(COTTUS_ERR_INVALID_ARGUMENT, "NULL pointer argument");
+    const int es = dtype_bytes(p->dtype);
+    if (!aligned(p->logits, es) || !aligned(p->uniforms, 4) || !aligned(p->temperature, 4) || !aligned(p->top_k, 4) ||
+        !aligned(p->top_p, 4) || !aligned(p->min_p, 4) || !aligned(p->tokens, 4) || !aligned(p->logprobs, 4))
+        return fail(COTTUS_ERR_INVALID_ARGUMENT, "a pointer is not aligned to its element");
+    const size_t b4 = (size_t)p->batch * 4;
+    const Span out[2] = {{p->tokens, b4}, {p->logprobs, p->logprobs ? b4 : 0}};
+    const Span in[6] = {{p->logits, (size_t)p->batch * p->vocab * es}, {p->uniforms, b4},
+                        {p->temperature, p->temperature ? b4 : 0}, {p->top_k, p->top_k ? b4 : 0},
+                        {p->top_p, p->top_p ? b4 : 0}, {p->min_p, p->min_p ? b4 : 0}};
+    bool clash = overlap(out[0], out[1]);
+    for (const Span& o : out)
+        for (const Span& i : in) clash = clash || overlap(o, i);
+    if (clash) return fail(COTTUS_ERR_INVALID_ARGUMENT, "an output overlaps another buffer");
+    SampleArgs a = {};
+    a.logits = p->logits;
+    a.uniforms = p->uniforms;
+    a.temperature = p->temperature;
+    a.top_k = p->top_k;
+    a.top_p = p->top_p;
+    a.min_p = p->min_p;
+    a.tokens = p->tokens;
+    a.logprobs = p->logprobs;
+    a.status = p->status;
+    a.vocab = p->vocab;
+    int bits = 1;
+    while ((int64_t(1) << bits) <= p->vocab) ++bits;
+    a.frac_bits = 62 - bits < 47 ? 62 - bits : 47;  // a weight fits three 16-bit limbs, a row's sum 62 bits
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const int sms = device_sm_count(dev);
+    // the smallest cluster that gives every SM work, and whose slices let two CTAs share an SM
+    int cluster = 1;
+    while (cluster < kMaxCluster &&
+           ((long long)p->batch * cluster < sms || sample_smem((p->vocab + cluster - 1) / cluster, es) > 114 * 1024))
+        cluster *= 2;
+    const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const cudaError_t e = p->dtype == COTTUS_F32   ? launch_sample<float>(a, p->batch, cluster, st)
+                          : p->dtype == COTTUS_F16 ? launch_sample<__half>(a, p->batch, cluster, st)
+                                                   : launch_sample<__nv_bfloat16>(a, p->batch, cluster, st);
+    return e == cudaSuccess ? COTTUS_OK : fail(COTTUS_ERR_CUDA, std::string("CUDA error: ") + cudaGetErrorString(e));
+}

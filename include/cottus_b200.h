@@ -49,8 +49,11 @@ enum cottus_status {
 #define COTTUS_STATUS_BAD_CONTEXT 0x2u  /* context < 0 or > max_blocks_per_seq * block_size */
 #define COTTUS_STATUS_BAD_POSITION 0x4u /* position outside the table / RoPE cache */
 #define COTTUS_STATUS_TIMEOUT 0x8u      /* a bounded wait inside a kernel gave up */
+#define COTTUS_STATUS_NO_TOKEN 0x10u    /* a row of logits holds no candidate (all -inf or NaN) */
 
-enum cottus_dtype { COTTUS_F32 = 0, COTTUS_F16 = 1 };
+/* COTTUS_BF16 and COTTUS_E4M3 are taken by cottus_rms_norm,
+ * cottus_quantize_fp8, cottus_fp8_linear and cottus_sample_tokens only. */
+enum cottus_dtype { COTTUS_F32 = 0, COTTUS_F16 = 1, COTTUS_BF16 = 2, COTTUS_E4M3 = 3 };
 
 /* Message of the last error returned on this host thread (mirrors the
  * reference's exception text where one exists). */
@@ -280,6 +283,118 @@ typedef struct {
 
 size_t cottus_o_proj_residual_workspace_size(const cottus_o_proj_params *p);
 int cottus_o_proj_residual(const cottus_o_proj_params *p, cottus_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * 8-bit activations and weights.  An e4m3 matrix comes with fp32 scales:
+ * element value = stored e4m3 value * its group's scale.
+ *   activations [rows][cols]: one scale per row and group of 128 columns,
+ *     stored group-major, scales[ceil(cols/128)][rows] (a matmul tile reads
+ *     the scales of its rows as one run);
+ *   weights [rows][cols]: one scale per block of 128 x 128,
+ *     scales[ceil(rows/128)][ceil(cols/128)].
+ * scale = max(amax / 448, 2^-126) with amax the group's largest |value|
+ * (448 = the largest e4m3 value); stored value = value / scale rounded to
+ * nearest even, at most 448 in magnitude.  A NaN anywhere in a group makes
+ * the group's scale and values NaN; an infinity makes the scale infinite,
+ * the infinities NaN and the finite values 0.
+ * Each call is one kernel, stream-ordered, without workspace; every call may
+ * be captured in a CUDA graph and replayed.  Buffers must not overlap unless
+ * a field says so.  rows or batch 0 is a successful no-op.
+ * ---------------------------------------------------------------------- */
+
+/* RMS norm with the residual's addition: h = x (+ residual), residual_out = h,
+ * y = h / sqrt(mean(h^2) + eps) * weight per row, in fp32.  Replaces
+ * residualAddCUDA followed by rmsnormCUDA (compute_primitives_cuda.cu:58-89;
+ * rmsnormCPU is the same formula).  y is written in out_dtype: fp32, fp16,
+ * bf16 (rounded once), or e4m3 with the row groups' scales. */
+typedef struct {
+    const void *x;         /* [rows][hidden], x_dtype (fp32, fp16, bf16) */
+    const float *residual; /* optional [rows][hidden] fp32 */
+    float *residual_out;   /* [rows][hidden] fp32, given with residual only; may be residual itself */
+    const float *weight;   /* [hidden] fp32 */
+    void *out;             /* [rows][hidden], out_dtype; may be x itself where the types have the same size */
+    float *scales;         /* e4m3 only: [ceil(hidden/128)][rows] */
+    int64_t rows;
+    int32_t hidden;
+    int32_t x_dtype;       /* enum cottus_dtype */
+    int32_t out_dtype;     /* enum cottus_dtype */
+    float eps;             /* >= 0 */
+} cottus_rms_norm_params;
+int cottus_rms_norm(const cottus_rms_norm_params *p, cottus_stream_t stream);
+
+/* x [rows][cols] (fp32, fp16, bf16) -> e4m3 with scales.  block_rows 1: the
+ * activation layout; 128: the weight layout.  No reference counterpart. */
+typedef struct {
+    const void *x;
+    void *out;          /* [rows][cols] e4m3 */
+    float *scales;      /* block_rows 1: [ceil(cols/128)][rows]; 128: [ceil(rows/128)][ceil(cols/128)] */
+    int64_t rows;
+    int32_t cols;
+    int32_t x_dtype;    /* enum cottus_dtype */
+    int32_t block_rows; /* 1 or 128 */
+} cottus_quantize_params;
+int cottus_quantize_fp8(const cottus_quantize_params *p, cottus_stream_t stream);
+
+/* Block-scaled e4m3 matrix product on the tensor cores:
+ *   out[m][n] = sum_b x_scales[b][m] * w_scales[n/128][b] *
+ *               sum_{k in group b} x[m][k] * weight[n][k]   (+ residual[m][n])
+ * with fp32 accumulation; x in the activation layout, weight ([out][in], as
+ * in cottus_o_proj_residual) in the weight layout.  in_features a multiple of
+ * 16, any out_features and any number of rows (a decode batch or a prefill
+ * chunk).  Replaces gemmCUDA (compute_primitives_cuda.cu:30-55) and, with
+ * residual, the residualAddCUDA after it (generic_transformer.cpp:305-325). */
+typedef struct {
+    const void *x;          /* [rows][in_features] e4m3, 16-B aligned */
+    const float *x_scales;  /* [ceil(in_features/128)][rows] */
+    const void *weight;     /* [out_features][in_features] e4m3, 16-B aligned */
+    const float *w_scales;  /* [ceil(out_features/128)][ceil(in_features/128)] */
+    const float *residual;  /* optional [rows][out_features] fp32; may be out itself when out_dtype is fp32 */
+    void *out;              /* [rows][out_features], out_dtype */
+    int32_t rows;
+    int32_t out_features;
+    int32_t in_features;
+    int32_t out_dtype;      /* COTTUS_F32, COTTUS_F16 or COTTUS_BF16 */
+    uint32_t *status;       /* optional device word */
+} cottus_fp8_linear_params;
+int cottus_fp8_linear(const cottus_fp8_linear_params *p, cottus_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * One token per row of logits.  Replaces the host argmax over the copied
+ * logits (engine.cpp:85-87), which temperature 0 reproduces.
+ * Per row, with the candidates (every logit but -inf and NaN) ordered by
+ * logit, largest first, equal logits by index, lowest first:
+ *   1. weights w_i = exp((logit_i - max) / temperature) (where the maximum
+ *      is +inf, its tokens weigh 1 and the others 0);
+ *   2. top-k: the first top_k candidates;
+ *   3. top-p: of those, the shortest run from the front whose weights sum to
+ *      at least top_p times their sum;
+ *   4. min-p: of those, the ones with w_i >= min_p (the largest weight is 1);
+ *      the front candidate always stays;
+ *   5. the token is the first one, in index order, at which the running sum
+ *      of the kept weights exceeds uniform * their sum.
+ * The weights are computed in fp64 and summed as 64-bit fixed-point numbers,
+ * so a result does not depend on the order of the additions.
+ * temperature <= 0 or NaN takes the front candidate.  top_k <= 0, top_p >= 1
+ * or NaN, min_p <= 0 or NaN switch that filter off; top_p <= 0 or min_p > 1
+ * keep the front candidate only.  uniform is clamped into [0, 1).  A row
+ * without a candidate gets token -1, log-probability -inf and
+ * COTTUS_STATUS_NO_TOKEN.  One kernel, no workspace, graph-replayable. */
+typedef struct {
+    const void *logits;       /* [batch][vocab], dtype */
+    const float *uniforms;    /* [batch] in [0, 1) */
+    const float *temperature; /* optional [batch]; NULL: 1 */
+    const int32_t *top_k;     /* optional [batch]; NULL: off */
+    const float *top_p;       /* optional [batch]; NULL: off */
+    const float *min_p;       /* optional [batch]; NULL: off */
+    int32_t *tokens;          /* [batch] */
+    float *logprobs;          /* optional [batch]: natural log of the token's share of the kept weights */
+    int32_t batch;
+    int32_t vocab;            /* at most COTTUS_MAX_VOCAB */
+    int32_t dtype;            /* COTTUS_F32, COTTUS_F16 or COTTUS_BF16 */
+    uint32_t *status;         /* optional device word */
+} cottus_sample_params;
+#define COTTUS_MAX_VOCAB 327680
+int cottus_sample_tokens(const cottus_sample_params *p, cottus_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Block-table gather: copies, bit for bit, the K and V rows of layer
