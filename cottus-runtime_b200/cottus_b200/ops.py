@@ -290,6 +290,8 @@ def attention_block(batch, x, w_qkv, w_o, residual, kv_pool, cos_sin, *, num_hea
 
 def _operand(t: torch.Tensor, name: str, shape, dtypes, device: int) -> int:
     """Checks one operand of the norm, 8-bit and sampling operators; its address."""
+    if t.get_device() == device and t.dtype in dtypes and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
     if not t.is_cuda:
@@ -298,9 +300,12 @@ def _operand(t: torch.Tensor, name: str, shape, dtypes, device: int) -> int:
         raise ValueError(f"{name} is on cuda:{t.get_device()}, the current device is cuda:{device}")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
+    raise ValueError(f"{name} must be contiguous")
+
+
+def _raw_stream(stream, device: int):
+    """The stream's handle; of the current stream without building a Stream object (3.4 us of a 13 us call)."""
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
 
 
 _ONLY_F32, _ONLY_I32, _ONLY_FP8 = (torch.float32,), (torch.int32,), (_FP8,)
@@ -328,20 +333,20 @@ def rms_norm(x, weight, *, eps=1e-5, residual=None, residual_out=None, out=None,
     elif residual_out is not None:
         raise ValueError("residual_out goes with residual")
     if out is None:
-        out = torch.empty((rows, hidden), dtype=out_dtype or x.dtype, device=x.device)
+        out = torch.empty_like(x, dtype=out_dtype)
     elif out_dtype is not None and out.dtype != out_dtype:
         raise TypeError(f"out is {out.dtype}, out_dtype is {out_dtype}")
     fp8 = out.dtype == _FP8
     p.out = _operand(out, "out", x.shape, _ONLY_FP8 if fp8 else _DT_WIDE, dev)
     if fp8:
         if scales is None:
-            scales = torch.empty(((hidden + 127) // 128, rows), dtype=torch.float32, device=x.device)
+            scales = x.new_empty(((hidden + 127) // 128, rows), dtype=torch.float32)
         p.scales = _operand(scales, "scales", ((hidden + 127) // 128, rows), _ONLY_F32, dev)
     elif scales is not None:
         raise ValueError("scales go with a torch.float8_e4m3fn output")
     p.rows, p.hidden, p.x_dtype, p.out_dtype = rows, hidden, _DT_WIDE[x.dtype], E4M3 if fp8 else _DT_WIDE[out.dtype]
     p.eps = eps
-    check(lib().cottus_rms_norm(C.byref(p), _stream(stream)))
+    check(lib().cottus_rms_norm(C.byref(p), _raw_stream(stream, dev)))
     return (out, scales) if fp8 else out
 
 
@@ -356,15 +361,15 @@ def quantize_fp8(x, *, block_rows=1, out=None, scales=None, stream=None):
     p = QuantizeParams()
     p.x = _operand(x, "x", x.shape, _DT_WIDE, dev)
     if out is None:
-        out = torch.empty((rows, cols), dtype=_FP8, device=x.device)
+        out = torch.empty_like(x, dtype=_FP8)
     groups = (cols + 127) // 128
     shape = ((rows + 127) // 128, groups) if block_rows == 128 else (groups, rows)
     if scales is None:
-        scales = torch.empty(shape, dtype=torch.float32, device=x.device)
+        scales = x.new_empty(shape, dtype=torch.float32)
     p.out = _operand(out, "out", x.shape, _ONLY_FP8, dev)
     p.scales = _operand(scales, "scales", shape, _ONLY_F32, dev)
     p.rows, p.cols, p.x_dtype, p.block_rows = rows, cols, _DT_WIDE[x.dtype], block_rows
-    check(lib().cottus_quantize_fp8(C.byref(p), _stream(stream)))
+    check(lib().cottus_quantize_fp8(C.byref(p), _raw_stream(stream, dev)))
     return out, scales
 
 
@@ -387,12 +392,12 @@ def fp8_linear(x, x_scales, weight, weight_scales, *, residual=None, out=None, o
     if residual is not None:
         p.residual = _operand(residual, "residual", (rows, fout), _ONLY_F32, dev)
     if out is None:
-        out = torch.empty((rows, fout), dtype=out_dtype, device=x.device)
+        out = x.new_empty((rows, fout), dtype=out_dtype)
     p.out = _operand(out, "out", (rows, fout), _DT_WIDE, dev)
     p.rows, p.out_features, p.in_features, p.out_dtype = rows, fout, fin, _DT_WIDE[out.dtype]
     if status is not None:
         p.status = _operand(status, "status", (1,), _ONLY_I32, dev)
-    check(lib().cottus_fp8_linear(C.byref(p), _stream(stream)))
+    check(lib().cottus_fp8_linear(C.byref(p), _raw_stream(stream, dev)))
     return out
 
 
@@ -420,16 +425,16 @@ def sample_tokens(logits, uniforms, *, temperature=None, top_k=None, top_p=None,
     if min_p is not None:
         p.min_p = _operand(min_p, "min_p", row, _ONLY_F32, dev)
     if out is None:
-        out = torch.empty(row, dtype=torch.int32, device=logits.device)
+        out = torch.empty_like(uniforms, dtype=torch.int32)
     p.tokens = _operand(out, "out", row, _ONLY_I32, dev)
     if return_logprobs and logprobs is None:
-        logprobs = torch.empty(row, dtype=torch.float32, device=logits.device)
+        logprobs = torch.empty_like(uniforms)
     if logprobs is not None:
         p.logprobs = _operand(logprobs, "logprobs", row, _ONLY_F32, dev)
     if status is not None:
         p.status = _operand(status, "status", (1,), _ONLY_I32, dev)
     p.batch, p.vocab, p.dtype = batch, vocab, _DT_WIDE[logits.dtype]
-    check(lib().cottus_sample_tokens(C.byref(p), _stream(stream)))
+    check(lib().cottus_sample_tokens(C.byref(p), _raw_stream(stream, dev)))
     return (out, logprobs) if return_logprobs else out
 
 

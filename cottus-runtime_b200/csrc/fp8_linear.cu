@@ -8,33 +8,45 @@
 //
 // The scales differ from group to group, so a group's 128-deep product is
 // accumulated in tensor memory (four tcgen05.mma of kind::f8f6f4, K = 32
-// each) and then added, scaled, to fp32 sums in registers.  CTA tile: 128
-// rows of x (the MMA's M) by BN rows of the weight (its N).  A row of x is a
+// each) and then added, scaled, to fp32 sums in registers.  A row of x is a
 // TMEM lane, so a thread's scale is one number for its whole run of columns:
-// one fused multiply-add per element and group.
+// one fused multiply-add per element and group.  Per CTA:
 //
 //   warps 0-7   the sums: warp w reads TMEM lanes 32 (w mod 4) .. + 31,
 //               columns BN/2 (w / 4) .. + BN/2
 //   warp 8      TMA producer (one thread): ring of stages, one group per stage
 //   warp 9      TMEM allocation and MMA issue (one thread)
+//   warps 10-11 scales: copy each group's row scales and weight scales to a
+//               ring of their own, kScaleBatch groups at once and kScaleSlots
+//               ahead (read by the sums themselves, one group ahead, a group
+//               took an L2 round trip; so it did with one 4-byte cp.async and
+//               one asynchronous arrival per group)
 //
-// TMEM holds 512 / BN product buffers, so the tensor cores work on the next
-// groups while a finished one is being added up.
+// TMEM holds two product buffers, so the tensor cores work on one group while
+// the other is being added up.
 //
-// A decode batch (rows <= 128) reads the weight once and is bound by HBM.
-// Where the weight has fewer tiles than the GPU has SMs, `splits` CTAs of one
-// cluster share a tile: each takes a contiguous run of groups, and the
-// partial sums meet in distributed shared memory, added in rank order, so a
-// result does not depend on timing.  Only the rows that exist are fetched
-// (the TMA box is as high as the batch, rounded up to 8); the remaining MMA
-// lanes read whatever follows in the same stage and their results are never
-// stored.
+// Two tiles:
+//   narrow  128 x 128, one CTA.  A decode batch (rows <= 128) reads the weight
+//           once and is bound by HBM or latency.  Where the weight has fewer
+//           tiles than the GPU has SMs, `splits` CTAs of one cluster share a
+//           tile: each takes a contiguous run of groups and sends its sums to
+//           the CTA that adds them (distributed shared memory, every CTA a
+//           share of the columns), in rank order, so a result does not depend
+//           on timing.  Only the rows that exist are fetched (the TMA box is
+//           as high as the batch, rounded up to 8); the other MMA lanes read
+//           whatever follows in the same stage and are never stored.
+//   wide    256 x 256 by a pair of CTAs (cta_group::2): each holds 128 rows of
+//           x and of the weight, and the pair's MMA reads both halves, so an
+//           SM moves 32 KB per 128 x 256 x 128 multiplies.  With the same
+//           128 x 256 per SM as one CTA (48 KB) shared memory was the limit,
+//           reads by the MMA and writes by TMA together: 1270 cycles a group
+//           against the 512 of the multiplies.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <atomic>
+#include <mutex>
 #include <string>
 
 #include "common.cuh"
@@ -49,20 +61,30 @@ int device_sm_count(int device);
 
 namespace {
 
-constexpr int kBM = 128;        // rows of x per tile
+constexpr int kBM = 128;        // rows of x per CTA
 constexpr int kBK = 128;        // elements (bytes) of k per stage: one scale group
+constexpr int kWRows = 128;     // rows of the weight per CTA and stage
 constexpr int kSumWarps = 8;    // warps that add up the groups
-constexpr int kThreads = (kSumWarps + 4) * 32;  // and one warpgroup for the producer and the MMA issue
+constexpr int kThreads = (kSumWarps + 4) * 32;  // and one warpgroup for the producer, the MMA issue and the scales
 // Registers per thread of the wide tile after the launch's even split: the
-// sums (128 per thread) take what the producer's warpgroup gives back.  The
-// launch must have brought that many (checked on the host).
-constexpr int kSumRegs = 232, kCtrlRegs = 40;
+// sums (128 per thread) take what the other warpgroup gives back.  The launch
+// must have brought that many (checked on the host).
+constexpr int kSumRegs = 224, kCtrlRegs = 56;
 constexpr int kMinLaunchRegs = (kSumRegs * kSumWarps * 32 + kCtrlRegs * 128 + kThreads - 1) / kThreads;
 constexpr int kMaxStages = 12;
 constexpr int kMaxSplits = 8;   // portable cluster size
+constexpr int kBufs = 2;        // product buffers in TMEM
 constexpr int kStagePitch = 20; // words per staged row of 16 columns (conflict-free 16-byte accesses)
-constexpr uint32_t kTmemCols = 512;
-constexpr size_t kSmemMax = 232448;  // dynamic shared memory per CTA, 227 KB
+constexpr int kScaleSlots = 3;  // of kScaleBatch groups each
+constexpr int kScaleBatch = 4;
+constexpr int kScaleWords = kBM + 4;  // a group's scales: 128 rows, then one per 128 columns of the tile
+constexpr size_t kSmemMax = 232448;   // dynamic shared memory per CTA, 227 KB
+// per sum warp: 32 rows of 128 bytes (wide, TMA stores), or of 16 padded columns
+template <bool PAIR>
+constexpr int kWarpStaging = PAIR ? 32 * 128 : 32 * kStagePitch * 4;
+// scales, barriers and words behind the ring and the staging area
+constexpr size_t kTailBytes =
+    (size_t)kScaleSlots * kScaleBatch * kScaleWords * 4 + (2 * kMaxStages + 2 * kBufs + 2 * kScaleSlots + 1) * 8 + 16 + 32 * 4;
 
 struct LinArgs {
     const float* xs;
@@ -70,7 +92,9 @@ struct LinArgs {
     const float* residual;
     void* out;
     uint32_t* status;
-    int M, N, groups, m_tiles, n_tiles, splits, stages, x_rows, out_dtype;
+    int M, N, groups, n_blocks, m_tiles, n_tiles, splits, stages, x_rows, out_dtype;
+    int staging_bytes;
+    int tma_out;  // whole 128-byte pieces of out may be stored by TMA
     int vec;  // rows of out and residual start on 16 bytes and hold whole runs of 4
 };
 
@@ -80,16 +104,59 @@ __device__ __forceinline__ uint64_t sw128_kmajor_desc(uint32_t smem_byte_addr) {
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 // kind::f8f6f4: e4m3 A and B (format 0), fp32 accumulator, both K-major.
-template <int BN>
+template <int M, int N>
 constexpr uint32_t f8_idesc() {
-    return (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+    return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Arrival on `bar` (of both CTAs of a pair) once this thread's multiplies so far are done.
+template <bool PAIR>
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::
+                         "r"(smem_addr(bar)), "h"((uint16_t)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                     : "memory");
 }
+template <bool PAIR>
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+            "l"(ad), "l"(bd), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+            "l"(ad), "l"(bd), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)), "r"(cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)), "r"(cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
+    if constexpr (PAIR)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+    else
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+// 32 columns of this warp's 32 lanes.
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
@@ -100,34 +167,88 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
           "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(addr));
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+// Waits for this warp's TMEM loads; v passes through, so that no use of it is
+// scheduled before the wait (30 operands are the most an asm statement takes).
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        asm volatile(""
+                     : "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]), "+r"(v[i + 5]),
+                       "+r"(v[i + 6]), "+r"(v[i + 7]));
 }
+
+// 2-D tiled TMA store from this CTA's shared memory, in the thread's bulk group.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(c0), "r"(c1), "r"(smem_addr(src))
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// The thread's stores have read their shared memory / are complete.
+__device__ __forceinline__ void tma_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-// 16 bytes of CTA `rank`'s shared memory at this CTA's address `local`.
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t local, uint32_t rank) {
+// Address of CTA `rank`'s copy of this CTA's shared-memory address.
+__device__ __forceinline__ uint32_t cluster_addr(const void* local, uint32_t rank) {
     uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(a)
-                 : "memory");
-    return v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(local)), "r"(rank));
+    return a;
 }
-
-__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t local, uint32_t rank) {
-    uint32_t a, v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
+__device__ __forceinline__ void st_cluster_f4(uint32_t a, float4 v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+                 : "memory");
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t a, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+__device__ __forceinline__ void st_shared_u4(uint32_t a, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// mbar_wait_bounded by a whole warp; the same answer in every lane.  (The
+// control warps run their loops with all lanes and elect one for the copies
+// and multiplies: with lane 0 alone in the loop every operand of those went
+// from a per-thread to a uniform register first, 800 cycles a group.)
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity) {
+    bool ok = mbar_try_wait(bar, parity);
+    if (__all_sync(0xffffffffu, ok)) return true;
+    const long long t0 = clock64();
+    bool all, late;
+    do {
+        ok = ok || mbar_try_wait(bar, parity);
+        all = __all_sync(0xffffffffu, ok);
+        late = __any_sync(0xffffffffu, clock64() - t0 > kWaitLimitCycles);
+    } while (!all && !late);
+    return all;
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(p));
+    return p != 0;
+}
+// First run of 4 columns that split q of a 128-wide tile sums up.
+__device__ __forceinline__ int first_run(int q, int splits) { return (q * 32 + splits - 1) / splits; }
+// 2-D tiled TMA load into this CTA's shared memory, completion counted on the
+// barrier at cluster address `bar` (of either CTA of the pair).
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
 }
 
 // Four sums of row m, columns n .. n + 3: residual added, rounded once, stored.
@@ -172,35 +293,43 @@ struct Ring {
     }
 };
 
-template <int BN>
-constexpr size_t lin_tail_bytes() {  // staging rows and barriers behind the ring
-    return (size_t)kSumWarps * 32 * kStagePitch * 4 + (2 * kMaxStages + 2 * (kTmemCols / BN) + 1) * 8 + 8;
-}
-
-template <int BN>
+// BN: columns of the tile (and of a product buffer).  PAIR: two CTAs share it
+// (the wide tile), else one CTA or a.splits of them (the narrow one).
+template <int BN, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_constant__ CUtensorMap xmap,
                                                                  const __grid_constant__ CUtensorMap wmap,
+                                                                 const __grid_constant__ CUtensorMap omap,
                                                                  const LinArgs a) {
-    constexpr int HALF = BN / 2, NBUF = kTmemCols / BN, PART_PITCH = BN + 4;
-    constexpr bool SPLIT = BN == 128;  // the wide tile is for products with tiles enough
-    const int splits = SPLIT ? a.splits : 1;
+    static_assert(BN == (PAIR ? 2 : 1) * kWRows, "a CTA brings 128 rows of the weight");
+    constexpr int HALF = BN / 2;
+    constexpr uint32_t TMEM_COLS = kBufs * BN;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const int stage_bytes = (a.x_rows + BN) * kBK;
+    const int stage_bytes = (a.x_rows + kWRows) * kBK;
     float* staging = reinterpret_cast<float*>(smem + (size_t)a.stages * stage_bytes);
-    uint64_t* full = reinterpret_cast<uint64_t*>(staging + kSumWarps * 32 * kStagePitch);
+    float* scales = staging + a.staging_bytes / 4;
+    uint64_t* full = reinterpret_cast<uint64_t*>(scales + kScaleSlots * kScaleBatch * kScaleWords);
     uint64_t* empty = full + kMaxStages;
     uint64_t* tm_full = empty + kMaxStages;
-    uint64_t* tm_empty = tm_full + NBUF;
-    uint64_t* done = tm_empty + NBUF;
+    uint64_t* tm_empty = tm_full + kBufs;
+    uint64_t* sc_full = tm_empty + kBufs;
+    uint64_t* sc_empty = sc_full + kScaleSlots;
+    uint64_t* done = sc_empty + kScaleSlots;
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(done + 1);
-    uint32_t* s_failed = s_tmem + 1;
+    uint32_t* s_failed = s_tmem + 1;  // a wait of this CTA ran out; one of the cluster did
+    uint32_t* s_run = s_tmem + 4;     // splits: where a run of 4 columns is summed up (cluster address)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = splits > 1 ? (int)cluster_rank() : 0;
-    const int first = blockIdx.x / splits, step = gridDim.x / splits;
+    const int splits = PAIR ? 1 : a.splits;
+    const int cluster = PAIR ? 2 : splits;
+    const int rank = cluster > 1 ? (int)cluster_rank() : 0;
+    const int first = blockIdx.x / cluster, step = gridDim.x / cluster;
     const int tiles = a.m_tiles * a.n_tiles;
     // this CTA's groups of every tile it works on
-    const int g0 = (int)((long long)a.groups * rank / splits), g1 = (int)((long long)a.groups * (rank + 1) / splits);
+    const int g0 = PAIR ? 0 : (int)((long long)a.groups * rank / splits);
+    const int g1 = PAIR ? a.groups : (int)((long long)a.groups * (rank + 1) / splits);
+    // first row of x, and first column, of tile t in this CTA
+    auto tile_m = [&](int t) { return PAIR ? (t % a.m_tiles * 2 + rank) * kBM : t % a.m_tiles * kBM; };
+    auto tile_n = [&](int t) { return t / a.m_tiles * BN; };
 
     if (threadIdx.x == 0) {
         prefetch_tensormap(&xmap);
@@ -209,24 +338,33 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < NBUF; ++i) {
+        for (int i = 0; i < kBufs; ++i) {
             mbar_init(&tm_full[i], 1);
-            mbar_init(&tm_empty[i], kSumWarps);
+            mbar_init(&tm_empty[i], (PAIR ? 2 : 1) * kSumWarps);
+        }
+        for (int i = 0; i < kScaleSlots; ++i) {
+            mbar_init(&sc_full[i], 2);
+            mbar_init(&sc_empty[i], kSumWarps);
         }
         mbar_init(done, 1);
         fence_barrier_init();
-        *s_failed = 0;
+        s_failed[0] = s_failed[1] = 0;
     }
-    if (warp == kSumWarps + 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(s_tmem)),
-                     "r"(kTmemCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (warp == kSumWarps + 1) tmem_alloc<PAIR>(s_tmem, TMEM_COLS);
+    if (!PAIR && splits > 1 && warp == kSumWarps + 2) {
+        // run r of 32 belongs to split r * splits / 32; its sums lie at
+        // [run][split][row] there, 16 bytes of padding per run
+        const int q = (lane * splits) >> 5;
+        s_run[lane] = cluster_addr(staging, q) + (lane - first_run(q, splits)) * (splits * a.x_rows + 1) * 16;
     }
     tc_before();
     __syncthreads();
     tc_after();
     const uint32_t tmem = *s_tmem;
+    // every CTA of the cluster has started and set up its barriers (a pair
+    // needs that now, splits before they send their sums)
+    if (cluster > 1) cluster_arrive();
+    if (PAIR) cluster_wait();
     grid_dependency_wait();
     // (after the allocation above: a dependent that also allocates TMEM can
     // then only wait for this grid, never the other way round)
@@ -234,129 +372,223 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
 
     bool ok = true;
     if (warp >= kSumWarps) {
-    if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
-    if (warp == kSumWarps) {
-        if (lane == 0) {
+        if constexpr (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
+        if (warp == kSumWarps) {
             // ---- producer ------------------------------------------------
             Ring r;
             int issued = 0;
             for (int t = first; t < tiles && ok; t += step) {
-                const int m0 = (t % a.m_tiles) * kBM, n0 = (t / a.m_tiles) * BN;
+                const int m0 = tile_m(t), w0 = tile_n(t) + (PAIR ? rank * kWRows : 0);
                 for (int g = g0; g < g1; ++g) {
-                    if (!mbar_wait_bounded(&empty[r.slot], r.phase ^ 1)) {
-                        ok = false;
-                        break;
+                    ok = mbar_wait_warp(&empty[r.slot], r.phase ^ 1);
+                    if (!ok) break;
+                    uint8_t* st = smem + r.slot * stage_bytes;
+                    if (elect_one()) {
+                        if constexpr (PAIR) {
+                            // the first CTA's barrier counts both CTAs' bytes
+                            const uint32_t bar = cluster_addr(&full[r.slot], 0);
+                            if (rank == 0) mbar_arrive_expect_tx(&full[r.slot], 2 * (uint32_t)stage_bytes);
+                            tma_load_2d_pair(st, &xmap, bar, g * kBK, m0);
+                            tma_load_2d_pair(st + a.x_rows * kBK, &wmap, bar, g * kBK, w0);
+                        } else {
+                            mbar_arrive_expect_tx(&full[r.slot], (uint32_t)stage_bytes);
+                            tma_load_2d(st, &xmap, &full[r.slot], g * kBK, m0);
+                            tma_load_2d(st + a.x_rows * kBK, &wmap, &full[r.slot], g * kBK, w0);
+                        }
                     }
-                    uint8_t* st = smem + (size_t)r.slot * stage_bytes;
-                    mbar_arrive_expect_tx(&full[r.slot], (uint32_t)stage_bytes);
-                    tma_load_2d(st, &xmap, &full[r.slot], g * kBK, m0);
-                    tma_load_2d(st + a.x_rows * kBK, &wmap, &full[r.slot], g * kBK, n0);
+                    __syncwarp();
                     ++issued;
                     r.next(a.stages);
                 }
             }
             if (!ok) {
-                // let this CTA's copies in flight land before it gives up
+                // let the copies in flight land before giving up (a pair's
+                // second CTA leaves it to the first, whose barriers count
+                // them, and waits for it at the end)
                 Ring q = r;
-                for (int i = 0; i < a.stages && i < issued; ++i) {
+                for (int i = 0; i < a.stages && i < issued && !(PAIR && rank); ++i) {
                     if (q.slot == 0) {
                         q.slot = a.stages;
                         q.phase ^= 1;
                     }
                     --q.slot;
-                    (void)mbar_wait_bounded(&full[q.slot], q.phase);
+                    (void)mbar_wait_warp(&full[q.slot], q.phase);
                 }
-                *s_failed = 1;
+                if (lane == 0) s_failed[0] = 1;
             }
-        }
-    } else if (warp == kSumWarps + 1) {
-        if (lane == 0) {
+        } else if (warp == kSumWarps + 1 && !(PAIR && rank)) {
             // ---- MMA issue -----------------------------------------------
-            constexpr uint32_t idesc = f8_idesc<BN>();
+            constexpr uint32_t idesc = f8_idesc<(PAIR ? 2 : 1) * kBM, BN>();
             Ring r, b;
             for (int t = first; t < tiles && ok; t += step) {
                 for (int g = g0; g < g1; ++g) {
-                    if (!mbar_wait_bounded(&tm_empty[b.slot], b.phase ^ 1) || !mbar_wait_bounded(&full[r.slot], r.phase)) {
-                        ok = false;
-                        break;
-                    }
+                    ok = mbar_wait_warp(&tm_empty[b.slot], b.phase ^ 1) && mbar_wait_warp(&full[r.slot], r.phase);
+                    if (!ok) break;
                     tc_after();
-                    const uint32_t xa = smem_addr(smem + (size_t)r.slot * stage_bytes), wa = xa + a.x_rows * kBK;
+                    const uint32_t xa = smem_addr(smem) + r.slot * stage_bytes, wa = xa + a.x_rows * kBK;
+                    const uint64_t ad = sw128_kmajor_desc(xa), bd = sw128_kmajor_desc(wa);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < kBK / 32; ++kk) {
-                        const uint64_t ad = sw128_kmajor_desc(xa + kk * 32), bd = sw128_kmajor_desc(wa + kk * 32);
-                        asm volatile(
-                            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(
-                                tmem + (uint32_t)(b.slot * BN)),
-                            "l"(ad), "l"(bd), "r"(idesc), "r"((uint32_t)kk)
-                            : "memory");
+                        for (int kk = 0; kk < kBK / 32; ++kk)  // (32 bytes further: 2 in units of 16)
+                            mma_f8<PAIR>(tmem + (uint32_t)(b.slot * BN), ad + 2 * kk, bd + 2 * kk, idesc, (uint32_t)kk);
+                        mma_commit<PAIR>(&empty[r.slot]);
+                        mma_commit<PAIR>(&tm_full[b.slot]);
                     }
-                    mma_commit(&empty[r.slot]);
-                    mma_commit(&tm_full[b.slot]);
+                    __syncwarp();
                     r.next(a.stages);
-                    b.next(NBUF);
+                    b.next(kBufs);
                 }
             }
             if (!ok) {
                 // every multiply issued so far ends before the memory is given back
-                mma_commit(done);
-                (void)mbar_wait_bounded(done, 0);
-                *s_failed = 1;
+                if (elect_one()) mma_commit<PAIR>(done);
+                __syncwarp();
+                (void)mbar_wait_warp(done, 0);
+                if (lane == 0) s_failed[0] = 1;
             }
+        } else if (warp >= kSumWarps + 2) {
+            // ---- scales: half of the rows each, kScaleBatch groups at once ----
+            const int part = warp - kSumWarps - 2;
+            Ring r;
+            for (int t = first; t < tiles && ok; t += step) {
+                const int m = tile_m(t) + part * 64 + lane, nb = tile_n(t) / 128 + lane;
+                const bool live0 = m < a.M, live1 = m + 32 < a.M;
+                const bool live_w = part == 0 && lane < BN / 128 && nb < a.n_blocks;
+                const float* xs = a.xs + m;
+                const float* ws = a.ws + (size_t)nb * a.groups;
+                for (int gb = g0; gb < g1 && ok; gb += kScaleBatch) {
+                    float v0[kScaleBatch], v1[kScaleBatch], w[kScaleBatch];
+#pragma unroll
+                    for (int j = 0; j < kScaleBatch; ++j) {
+                        const int g = gb + j;
+                        v0[j] = live0 && g < g1 ? xs[(size_t)g * a.M] : 0.f;
+                        v1[j] = live1 && g < g1 ? xs[(size_t)g * a.M + 32] : 0.f;
+                        w[j] = live_w && g < g1 ? ws[g] : 0.f;
+                    }
+                    ok = mbar_wait_warp(&sc_empty[r.slot], r.phase ^ 1);
+                    if (!ok) break;
+#pragma unroll
+                    for (int j = 0; j < kScaleBatch; ++j) {
+                        float* dst = scales + (r.slot * kScaleBatch + j) * kScaleWords;
+                        dst[part * 64 + lane] = v0[j];
+                        dst[part * 64 + lane + 32] = v1[j];
+                        if (part == 0 && lane < BN / 128) dst[kBM + lane] = w[j];
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sc_full[r.slot]);
+                    r.next(kScaleSlots);
+                }
+            }
+            if (!ok && lane == 0) s_failed[0] = 1;
         }
-    }
+        __syncwarp();
+        if (!PAIR && cluster > 1) cluster_wait();
     } else {
-        if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
+        if constexpr (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
         // ---- sums ----------------------------------------------------------
         const int quad = warp & 3, half = warp >> 2;
         const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * HALF);
-        float* stg = staging + warp * 32 * kStagePitch;
-        Ring b;
+        uint8_t* stg = reinterpret_cast<uint8_t*>(staging) + warp * kWarpStaging<PAIR>;
+        if (!PAIR && cluster > 1) cluster_wait();
+        Ring b, r;
         for (int t = first; t < tiles && ok; t += step) {
-            const int m0 = (t % a.m_tiles) * kBM, n0 = (t / a.m_tiles) * BN;
-            const int m = m0 + quad * 32 + lane, nh = n0 + half * HALF;
-            const bool rows_live = m0 + quad * 32 < a.M;  // (uniform in the warp)
-            const float* xs = a.xs + (m < a.M ? m : 0);
-            const float* ws = a.ws + (size_t)((nh < a.N ? nh : 0) / 128) * a.groups;
-            float acc[HALF];
+            const int m0 = tile_m(t) + quad * 32, nh = tile_n(t) + half * HALF;
+            const bool rows_live = m0 < a.M;  // (uniform in the warp)
+            float2 acc[HALF / 2];
 #pragma unroll
-            for (int c = 0; c < HALF; ++c) acc[c] = 0.f;
-            float sx = g0 < g1 ? xs[(size_t)g0 * a.M] : 0.f, sw = g0 < g1 ? ws[g0] : 0.f;
+            for (int c = 0; c < HALF / 2; ++c) acc[c] = make_float2(0.f, 0.f);
             for (int g = g0; g < g1; ++g) {
-                const float s = sx * sw;
-                if (g + 1 < g1) {
-                    sx = xs[(size_t)(g + 1) * a.M];
-                    sw = ws[g + 1];
-                }
-                ok = ok && mbar_wait_bounded(&tm_full[b.slot], b.phase);
-                ok = __all_sync(0xffffffffu, ok);
+                const int j = (g - g0) % kScaleBatch;
+                if (j == 0) ok = mbar_wait_warp(&sc_full[r.slot], r.phase);
+                ok = ok && mbar_wait_warp(&tm_full[b.slot], b.phase);
                 if (!ok) break;
                 tc_after();
+                const float* sc = scales + (r.slot * kScaleBatch + j) * kScaleWords;
+                const float s = sc[quad * 32 + lane] * sc[kBM + (BN > 128 ? half : 0)];
                 if (rows_live) {
+                    // the next 32 columns are on their way while these are added
+                    // (a load takes about 75 cycles whatever its width: with
+                    // 16 columns at a time a group took 600)
+                    const float2 s2 = make_float2(s, s);
+                    uint32_t v[2][32];
+                    const uint32_t at = taddr + (uint32_t)(b.slot * BN);
+                    tmem_ld32(at, v[0]);
 #pragma unroll
-                    for (int c0 = 0; c0 < HALF; c0 += 32) {
-                        uint32_t v[32];
-                        tmem_ld32(taddr + (uint32_t)(b.slot * BN + c0), v);
-                        tmem_wait_ld();
+                    for (int i = 0; i < HALF / 32; ++i) {
+                        tmem_wait_ld(v[i & 1]);
+                        if (i + 1 < HALF / 32) tmem_ld32(at + (uint32_t)(i + 1) * 32, v[(i + 1) & 1]);
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) acc[c0 + c] = fmaf(s, __uint_as_float(v[c]), acc[c0 + c]);
+                        for (int c = 0; c < 16; ++c)
+                            acc[i * 16 + c] = ffma2(
+                                make_float2(__uint_as_float(v[i & 1][2 * c]), __uint_as_float(v[i & 1][2 * c + 1])), s2,
+                                acc[i * 16 + c]);
                     }
                 }
                 tc_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&tm_empty[b.slot]);
-                b.next(NBUF);
+                const bool last = j == kScaleBatch - 1 || g + 1 == g1;
+                if (lane == 0) {
+                    if (PAIR && rank) mbar_arrive_cluster(cluster_addr(&tm_empty[b.slot], 0));
+                    else mbar_arrive(&tm_empty[b.slot]);
+                    if (last) mbar_arrive(&sc_empty[r.slot]);
+                }
+                b.next(kBufs);
+                if (last) r.next(kScaleSlots);
             }
             if (!ok) break;
-            if (splits > 1) {
-                // the only tile of this cluster: its ring is idle (every stage
-                // has been multiplied), so it takes the partial sums
-                float* part = reinterpret_cast<float*>(smem) + (size_t)(quad * 32 + lane) * PART_PITCH + half * HALF;
-                if (m < a.M) {
+            if (!PAIR && splits > 1) {
+                // (the only tile of this cluster) every run of 4 columns goes to
+                // the CTA that sums it up
+                if (m0 + lane < a.M) {
+                    const uint32_t mine = (uint32_t)(rank * a.x_rows + quad * 32 + lane) * 16;
 #pragma unroll
                     for (int c = 0; c < HALF; c += 4)
-                        *reinterpret_cast<float4*>(part + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+                        st_cluster_f4(s_run[(half * HALF + c) / 4] + mine,
+                                      make_float4(acc[c / 2].x, acc[c / 2].y, acc[c / 2 + 1].x, acc[c / 2 + 1].y));
+                }
+            } else if (PAIR && a.tma_out) {
+                // 128 bytes of each of the warp's rows at a time, swizzled as
+                // the tensor map has it, stored by TMA (which drops what lies
+                // past the last row or column)
+                if (rows_live) {
+                    const uint32_t row = smem_addr(stg) + lane * 128;
+                    const uint32_t swz = lane & 7;
+                    if (a.out_dtype == COTTUS_F32) {
+#pragma unroll
+                        for (int c0 = 0; c0 < HALF; c0 += 32) {
+                            if (lane == 0) tma_store_read();
+                            __syncwarp();
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const float2 u = acc[c0 / 2 + 2 * j], w = acc[c0 / 2 + 2 * j + 1];
+                                st_shared_u4(row + ((j ^ swz) << 4), make_uint4(__float_as_uint(u.x), __float_as_uint(u.y),
+                                                                               __float_as_uint(w.x), __float_as_uint(w.y)));
+                            }
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0 && nh + c0 < a.N) tma_store_2d(&omap, stg, (nh + c0) * 4, m0);
+                        }
+                    } else {
+                        const bool f16 = a.out_dtype == COTTUS_F16;
+#pragma unroll
+                        for (int c0 = 0; c0 < HALF; c0 += 64) {
+                            if (lane == 0) tma_store_read();
+                            __syncwarp();
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                uint32_t p[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const float2 u = acc[c0 / 2 + 4 * j + e];
+                                    p[e] = f16 ? pack_h2(u.x, u.y) : pack_bf2(u.x, u.y);
+                                }
+                                st_shared_u4(row + ((j ^ swz) << 4), make_uint4(p[0], p[1], p[2], p[3]));
+                            }
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0 && nh + c0 < a.N) tma_store_2d(&omap, stg, (nh + c0) * 2, m0);
+                        }
+                    }
                 }
             } else if (rows_live) {
                 // 16 columns at a time through shared memory, so that four
@@ -366,110 +598,159 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
                     __syncwarp();
 #pragma unroll
                     for (int c = 0; c < 16; c += 4)
-                        *reinterpret_cast<float4*>(stg + lane * kStagePitch + c) =
-                            make_float4(acc[c0 + c], acc[c0 + c + 1], acc[c0 + c + 2], acc[c0 + c + 3]);
+                        *reinterpret_cast<float4*>(reinterpret_cast<float*>(stg) + lane * kStagePitch + c) =
+                            make_float4(acc[(c0 + c) / 2].x, acc[(c0 + c) / 2].y, acc[(c0 + c) / 2 + 1].x,
+                                        acc[(c0 + c) / 2 + 1].y);
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int rr = i * 8 + (lane >> 2), mm = m0 + quad * 32 + rr, n = nh + c0 + (lane & 3) * 4;
-                        const float4 v = *reinterpret_cast<const float4*>(stg + rr * kStagePitch + (lane & 3) * 4);
-                        if (mm < a.M && n < a.N) store_out4(a, mm, n, v);
+                        const int rr = i * 8 + (lane >> 2), n = nh + c0 + (lane & 3) * 4;
+                        const float4 v =
+                            *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(stg) + rr * kStagePitch + (lane & 3) * 4);
+                        if (m0 + rr < a.M && n < a.N) store_out4(a, m0 + rr, n, v);
                     }
                 }
             }
         }
-        if (!ok && lane == 0) *s_failed = 1;
+        if (PAIR && lane == 0) tma_store_done();
+        if (!ok && lane == 0) s_failed[0] = 1;
     }
     __syncwarp();
-    if (splits > 1) {
-        cluster_sync_all();  // every CTA's partial sums are in its shared memory
-        const int m0 = (first % a.m_tiles) * kBM, n0 = (first / a.m_tiles) * BN;
-        const int rows = a.M - m0 < kBM ? a.M - m0 : kBM;
-        uint32_t failed = 0;
-        for (int q = 0; q < splits; ++q) failed |= ld_cluster_u32(smem_addr(s_failed), q);
-        if (!failed) {
-            for (int i = rank * kThreads + threadIdx.x; i < rows * (BN / 4); i += splits * kThreads) {
-                const int r = i / (BN / 4), c = (i % (BN / 4)) * 4;
-                if (n0 + c >= a.N) continue;
-                const uint32_t at = smem_addr(reinterpret_cast<float*>(smem) + (size_t)r * PART_PITCH + c);
-                float4 p[kMaxSplits];
-#pragma unroll
-                for (int q = 0; q < kMaxSplits; ++q)
-                    if (q < splits) p[q] = ld_cluster_f4(at, q);
-                float4 v = p[0];
-#pragma unroll
-                for (int q = 1; q < kMaxSplits; ++q)
-                    if (q < splits) {
-                        v.x += p[q].x;
-                        v.y += p[q].y;
-                        v.z += p[q].z;
-                        v.w += p[q].w;
+    if (!PAIR && splits > 1) {
+        __syncthreads();
+        if (threadIdx.x < splits && s_failed[0]) st_cluster_u32(cluster_addr(s_failed + 1, threadIdx.x), 1u);
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();  // every CTA's partial sums are where they are added
+        if (!s_failed[1]) {
+            const int m0 = tile_m(first), n0 = tile_n(first);
+            const int rows = a.M - m0 < kBM ? a.M - m0 : kBM;
+            const int run0 = first_run(rank, splits), runs = first_run(rank + 1, splits) - run0;
+            const int sh = runs > 16 ? 5 : (runs > 8 ? 4 : (runs > 4 ? 3 : 2));  // lanes per row
+            const int run = threadIdx.x & ((1 << sh) - 1), n = n0 + (run0 + run) * 4;
+            if (run < runs && n < a.N) {
+                const float4* p = reinterpret_cast<const float4*>(staging) + run * (splits * a.x_rows + 1);
+                for (int row = threadIdx.x >> sh; row < rows; row += kThreads >> sh) {
+                    float4 v = p[row];
+                    for (int q = 1; q < splits; ++q) {
+                        const float4 w = p[q * a.x_rows + row];
+                        v.x += w.x;
+                        v.y += w.y;
+                        v.z += w.z;
+                        v.w += w.w;
                     }
-                store_out4(a, m0 + r, n0 + c, v);
+                    store_out4(a, m0 + row, n, v);
+                }
             }
         }
-        cluster_sync_all();  // nobody leaves while its shared memory is being read
     }
     tc_before();
     __syncthreads();
-    if (threadIdx.x == 0 && *s_failed) report(a.status, COTTUS_STATUS_TIMEOUT);
-    if (warp == kSumWarps + 1)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    if (PAIR) {  // neither CTA leaves while the other's multiplies and arrivals may reach it
+        cluster_arrive();
+        cluster_wait();
+    }
+    if (threadIdx.x == 0 && s_failed[0]) report(a.status, COTTUS_STATUS_TIMEOUT);
+    if (warp == kSumWarps + 1) tmem_free<PAIR>(tmem, TMEM_COLS);
 }
 
 int fail(int code, const std::string& msg) { return set_error(code, msg); }
 
-// Once per device: the shared-memory limit, and the register count that the
-// wide tile's redistribution relies on.
-template <int BN>
-cudaError_t prepare_kernel() {
-    static std::atomic<uint64_t> ready{0};  // a bit per device
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 64 && (ready.load(std::memory_order_acquire) >> dev & 1)) return cudaSuccess;
-    auto kern = fp8_linear_kernel<BN>;
+// What a device allows, found at its first call.
+struct DeviceLimits {
+    int sms = 0;
+    int clusters[kMaxSplits + 1] = {};  // narrow-tile clusters of each size that are resident at once
+    int pairs = 0;                      // and wide-tile pairs (not every SM has a partner)
+    cudaError_t err = cudaSuccess;
+};
+template <int BN, bool PAIR>
+cudaError_t set_up_kernel() {
+    auto kern = fp8_linear_kernel<BN, PAIR>;
     cudaFuncAttributes fa = {};
-    e = cudaFuncGetAttributes(&fa, kern);
+    cudaError_t e = cudaFuncGetAttributes(&fa, kern);
     if (e != cudaSuccess) return e;
-    if (BN == 256 && fa.numRegs < kMinLaunchRegs) return cudaErrorInvalidConfiguration;
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
-    if (e == cudaSuccess && dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
-    return e;
+    // (a warp is given registers in steps of 8 per thread)
+    if (PAIR && (fa.numRegs + 7) / 8 * 8 < kMinLaunchRegs) return cudaErrorInvalidConfiguration;
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
+}
+DeviceLimits find_limits(int dev) {
+    DeviceLimits l;
+    l.sms = device_sm_count(dev);
+    l.err = set_up_kernel<128, false>();
+    if (l.err == cudaSuccess) l.err = set_up_kernel<256, true>();
+    auto resident = [&](auto kern, int size, int* n) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(size);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = kSmemMax;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = size;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (l.err == cudaSuccess) l.err = cudaOccupancyMaxActiveClusters(n, kern, &cfg);
+    };
+    for (int s = 1; s <= kMaxSplits; ++s) resident(fp8_linear_kernel<128, false>, s, &l.clusters[s]);
+    resident(fp8_linear_kernel<256, true>, 2, &l.pairs);
+    return l;
+}
+constexpr int kMaxDevices = 64;
+cudaError_t limits(DeviceLimits& l) {
+    static DeviceLimits cache[kMaxDevices];
+    static std::once_flag once[kMaxDevices];
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= kMaxDevices) return cudaErrorInvalidDevice;
+    std::call_once(once[dev], [&] { cache[dev] = find_limits(dev); });
+    l = cache[dev];
+    return l.err;
 }
 
-template <int BN>
+template <int BN, bool PAIR>
 cudaError_t launch_linear(const cottus_fp8_linear_params* p, LinArgs a, int grid, cudaStream_t st) {
     cudaError_t err = cudaSuccess;
     a.x_rows = p->rows < kBM ? (p->rows + 7) / 8 * 8 : kBM;
-    const size_t stage = (size_t)(a.x_rows + BN) * kBK;
-    const size_t room = kSmemMax - 1024 - lin_tail_bytes<BN>();
-    a.stages = (int)(room / stage);
+    a.staging_bytes = kSumWarps * kWarpStaging<PAIR>;
+    if (a.splits > 1) a.staging_bytes = (32 + a.splits - 1) / a.splits * (a.splits * a.x_rows + 1) * 16;
+    const size_t stage = (size_t)(a.x_rows + kWRows) * kBK;
+    const size_t rest = 1024 + (size_t)a.staging_bytes + kTailBytes;
+    a.stages = (int)((kSmemMax - rest) / stage);
     if (a.stages > kMaxStages) a.stages = kMaxStages;
+    // no more stages than a split has groups: a launch that needs little
+    // shared memory can become resident beside the one before it
+    const int most = (a.groups + a.splits - 1) / a.splits;
+    if (a.splits > 1 && a.stages > most) a.stages = most;
     const CUtensorMap xmap = make_tensor_map_2d_u8(p->x, p->in_features, p->rows, p->in_features, kBK, a.x_rows, true, &err);
     if (err != cudaSuccess) return err;
-    const CUtensorMap wmap = make_tensor_map_2d_u8(p->weight, p->in_features, p->out_features, p->in_features, kBK, BN,
-                                                   true, &err);
+    const CUtensorMap wmap =
+        make_tensor_map_2d_u8(p->weight, p->in_features, p->out_features, p->in_features, kBK, kWRows, true, &err);
     if (err != cudaSuccess) return err;
-    auto kern = fp8_linear_kernel<BN>;
-    const size_t smem = (size_t)a.stages * stage + lin_tail_bytes<BN>() + 1024;
-    err = prepare_kernel<BN>();
-    if (err != cudaSuccess) return err;
+    CUtensorMap omap = wmap;  // (not read without tma_out)
+    const int es = dtype_bytes(p->out_dtype);
+    a.tma_out = PAIR && !p->residual && aligned(p->out, 16) && (size_t)p->out_features * es % 16 == 0;
+    if (a.tma_out) {
+        omap = make_tensor_map_2d_u8(p->out, (uint64_t)p->out_features * es, p->rows, (uint64_t)p->out_features * es, 128, 32,
+                                     true, &err);
+        if (err != cudaSuccess) return err;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = rest + (size_t)a.stages * stage;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = a.splits;
+    attr[1].val.clusterDim.x = PAIR ? 2 : a.splits;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = a.splits > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kern, xmap, wmap, a);
+    cfg.numAttrs = PAIR || a.splits > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, fp8_linear_kernel<BN, PAIR>, xmap, wmap, omap, a);
 }
 
 }  // namespace
@@ -507,30 +788,30 @@ extern "C" int cottus_fp8_linear(const cottus_fp8_linear_params* p, cottus_strea
     a.M = M;
     a.N = N;
     a.groups = groups;
+    a.n_blocks = (N + 127) / 128;
     a.out_dtype = p->out_dtype;
     a.vec = N % 4 == 0 && aligned(p->out, es * 4) && aligned(p->residual, 16);
-    a.m_tiles = (M + kBM - 1) / kBM;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const int sms = device_sm_count(dev);
-    const int n256 = (N + 255) / 256, n128 = (N + 127) / 128;
+    DeviceLimits dev;
+    cudaError_t e = limits(dev);
+    if (e != cudaSuccess) return fail(COTTUS_ERR_CUDA, std::string("CUDA error: ") + cudaGetErrorString(e));
+    const int64_t narrow = (int64_t)((M + 127) / 128) * ((N + 127) / 128), wide = (int64_t)((M + 255) / 256) * ((N + 255) / 256);
+    if (narrow >= (int64_t(1) << 30)) return fail(COTTUS_ERR_UNSUPPORTED, "product too large");
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    cudaError_t e;
-    if ((long long)a.m_tiles * n128 >= (int64_t(1) << 30)) return fail(COTTUS_ERR_UNSUPPORTED, "product too large");
-    if (a.m_tiles > 1 && (long long)a.m_tiles * n256 >= sms) {
-        // enough tiles for every SM: the wide tile reads a third less shared memory per multiply
-        a.n_tiles = n256;
+    if (M > 128 && dev.pairs > 0 && wide >= dev.pairs) {
+        // enough tiles for every SM
+        a.m_tiles = (M + 255) / 256;
+        a.n_tiles = (N + 255) / 256;
         a.splits = 1;
-        const int tiles = a.m_tiles * n256;
-        e = launch_linear<256>(p, a, tiles < sms ? tiles : sms, st);
+        e = launch_linear<256, true>(p, a, 2 * (int)(wide < dev.pairs ? wide : dev.pairs), st);
     } else {
-        a.n_tiles = n128;
-        const int tiles = a.m_tiles * n128;
-        int s = tiles < sms ? sms / tiles : 1;
-        if (s > kMaxSplits) s = kMaxSplits;
-        if (s > groups) s = groups;
-        a.splits = s;
-        e = launch_linear<128>(p, a, s > 1 ? tiles * s : (tiles < sms ? tiles : sms), st);
+        a.m_tiles = (M + 127) / 128;
+        a.n_tiles = (N + 127) / 128;
+        // as many splits as leave all clusters resident at once
+        a.splits = 1;
+        for (int s = 2; s <= kMaxSplits && s <= groups; ++s)
+            if (narrow <= dev.clusters[s]) a.splits = s;
+        e = launch_linear<128, false>(p, a, a.splits > 1 ? (int)narrow * a.splits : (int)(narrow < dev.sms ? narrow : dev.sms),
+                                      st);
     }
     return e == cudaSuccess ? COTTUS_OK : fail(COTTUS_ERR_CUDA, std::string("CUDA error: ") + cudaGetErrorString(e));
 }

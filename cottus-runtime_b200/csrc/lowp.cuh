@@ -89,11 +89,34 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// Eight of them.  The quotients are correctly rounded: q0 = v * RN(1/s) is
+// within an ulp, and q0 + RN(v - q0 s) RN(1/s) is then RN(v / s) (Markstein,
+// IBM J. Res. Dev. 34, 1990), while nothing underflows: v below 2^-10 s is
+// 0 in e4m3 whatever its last bit, and for larger v the remainder stays a
+// normal number where s >= 2^-90.  Smaller, infinite and NaN scales divide.
+// Three packed operations for two quotients instead of two divisions: the
+// 28672 x 8200 bf16 weight took 272 us with divisions.
 __device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float s) {
-    uint2 r;
-    r.x = e4m3x2(__fdiv_rn(v[0], s), __fdiv_rn(v[1], s)) | (e4m3x2(__fdiv_rn(v[2], s), __fdiv_rn(v[3], s)) << 16);
-    r.y = e4m3x2(__fdiv_rn(v[4], s), __fdiv_rn(v[5], s)) | (e4m3x2(__fdiv_rn(v[6], s), __fdiv_rn(v[7], s)) << 16);
-    return r;
+    float q[8];
+    if (s >= 0x1p-90f && s < INFINITY) {
+        const float r = __frcp_rn(s);
+        const float2 r2 = make_float2(r, r), ns2 = make_float2(-s, -s);
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const float2 x = make_float2(v[j], v[j + 1]);
+            const float2 q0 = fmul2(x, r2);
+            const float2 q1 = ffma2(ffma2(q0, ns2, x), r2, q0);
+            q[j] = q1.x;
+            q[j + 1] = q1.y;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = __fdiv_rn(v[j], s);
+    }
+    uint2 o;
+    o.x = e4m3x2(q[0], q[1]) | (e4m3x2(q[2], q[3]) << 16);
+    o.y = e4m3x2(q[4], q[5]) | (e4m3x2(q[6], q[7]) << 16);
+    return o;
 }
 __device__ __forceinline__ uint8_t e4m3(float v, float s) { return (uint8_t)(e4m3x2(__fdiv_rn(v, s), 0.f) & 0xFFu); }
 
