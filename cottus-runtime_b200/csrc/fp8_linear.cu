@@ -73,18 +73,16 @@ constexpr int kSumRegs = 224, kCtrlRegs = 56;
 constexpr int kMinLaunchRegs = (kSumRegs * kSumWarps * 32 + kCtrlRegs * 128 + kThreads - 1) / kThreads;
 constexpr int kMaxStages = 12;
 constexpr int kMaxSplits = 8;   // portable cluster size
-constexpr int kBufs = 2;        // product buffers in TMEM
+constexpr int kMaxBufs = 4;     // product buffers in TMEM
 constexpr int kStagePitch = 20; // words per staged row of 16 columns (conflict-free 16-byte accesses)
 constexpr int kScaleSlots = 3;  // of kScaleBatch groups each
 constexpr int kScaleBatch = 4;
 constexpr int kScaleWords = kBM + 4;  // a group's scales: 128 rows, then one per 128 columns of the tile
 constexpr size_t kSmemMax = 232448;   // dynamic shared memory per CTA, 227 KB
-// per sum warp: 32 rows of 128 bytes (wide, TMA stores), or of 16 padded columns
-template <bool PAIR>
-constexpr int kWarpStaging = PAIR ? 32 * 128 : 32 * kStagePitch * 4;
+constexpr int kWarpStaging = 32 * 128;  // per sum warp: 128 bytes of each of its rows (or 16 padded columns)
 // scales, barriers and words behind the ring and the staging area
 constexpr size_t kTailBytes =
-    (size_t)kScaleSlots * kScaleBatch * kScaleWords * 4 + (2 * kMaxStages + 2 * kBufs + 2 * kScaleSlots + 1) * 8 + 16 + 32 * 4;
+    (size_t)kScaleSlots * kScaleBatch * kScaleWords * 4 + (2 * kMaxStages + 2 * kMaxBufs + 2 * kScaleSlots + 1) * 8 + 16 + 32 * 4;
 
 struct LinArgs {
     const float* xs;
@@ -113,13 +111,13 @@ __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_
 
 // Arrival on `bar` (of both CTAs of a pair) once this thread's multiplies so far are done.
 template <bool PAIR>
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
     if constexpr (PAIR)
         asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::
-                         "r"(smem_addr(bar)), "h"((uint16_t)3)
+                         "r"(bar), "h"((uint16_t)3)
                      : "memory");
     else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
                      : "memory");
 }
 template <bool PAIR>
@@ -138,13 +136,13 @@ __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t ad, uint64_t bd, uin
             : "memory");
 }
 template <bool PAIR>
-__device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
+__device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t cols) {
     if constexpr (PAIR) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)), "r"(cols)
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     } else {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)), "r"(cols)
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -179,10 +177,10 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[32]) {
 }
 
 // 2-D tiled TMA store from this CTA's shared memory, in the thread's bulk group.
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int c0, int c1) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
                      reinterpret_cast<uint64_t>(map)),
-                 "r"(c0), "r"(c1), "r"(smem_addr(src))
+                 "r"(c0), "r"(c1), "r"(src)
                  : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
@@ -197,10 +195,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-// Address of CTA `rank`'s copy of this CTA's shared-memory address.
-__device__ __forceinline__ uint32_t cluster_addr(const void* local, uint32_t rank) {
+// Address of CTA `rank`'s copy of a shared-memory address.
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t local, uint32_t rank) {
     uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(local)), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
     return a;
 }
 __device__ __forceinline__ void st_cluster_f4(uint32_t a, float4 v) {
@@ -213,24 +211,65 @@ __device__ __forceinline__ void st_cluster_u32(uint32_t a, uint32_t v) {
 __device__ __forceinline__ void st_shared_u4(uint32_t a, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// Arrival at shared-memory (PAIR: cluster) address `bar`, of a warp that has
+// finished reading: nothing it wrote has to become visible with it.
+template <bool PAIR>
+__device__ __forceinline__ void mbar_release(uint32_t bar) {
+    if constexpr (PAIR) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    else asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Barrier operations on 32-bit shared-memory addresses (64-bit pointers cost
+// the sums registers that they need for their accumulators).
+// (the thread may sleep up to a millisecond in each try, so that waiting warps
+// leave the issue slots to the sums)
+__device__ __forceinline__ bool bar_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(1000000u)
+        : "memory");
+    return ok != 0;
 }
 // mbar_wait_bounded by a whole warp; the same answer in every lane.  (The
 // control warps run their loops with all lanes and elect one for the copies
 // and multiplies: with lane 0 alone in the loop every operand of those went
 // from a per-thread to a uniform register first, 800 cycles a group.)
-__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity) {
-    bool ok = mbar_try_wait(bar, parity);
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+    bool ok = bar_try_wait(bar, parity);
     if (__all_sync(0xffffffffu, ok)) return true;
     const long long t0 = clock64();
     bool all, late;
     do {
-        ok = ok || mbar_try_wait(bar, parity);
+        ok = ok || bar_try_wait(bar, parity);
         all = __all_sync(0xffffffffu, ok);
         late = __any_sync(0xffffffffu, clock64() - t0 > kWaitLimitCycles);
     } while (!all && !late);
     return all;
+}
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ float ld_shared_f(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_shared_f4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_shared_f(uint32_t a, float v) {
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -243,12 +282,20 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ int first_run(int q, int splits) { return (q * 32 + splits - 1) / splits; }
 // 2-D tiled TMA load into this CTA's shared memory, completion counted on the
 // barrier at cluster address `bar` (of either CTA of the pair).
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
-        " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_addr(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
-        : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    if constexpr (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
+            " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+            : "memory");
 }
 
 // Four sums of row m, columns n .. n + 3: residual added, rounded once, stored.
@@ -302,24 +349,30 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
                                                                  const LinArgs a) {
     static_assert(BN == (PAIR ? 2 : 1) * kWRows, "a CTA brings 128 rows of the weight");
     constexpr int HALF = BN / 2;
-    constexpr uint32_t TMEM_COLS = kBufs * BN;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const int stage_bytes = (a.x_rows + kWRows) * kBK;
-    float* staging = reinterpret_cast<float*>(smem + (size_t)a.stages * stage_bytes);
-    float* scales = staging + a.staging_bytes / 4;
-    uint64_t* full = reinterpret_cast<uint64_t*>(scales + kScaleSlots * kScaleBatch * kScaleWords);
-    uint64_t* empty = full + kMaxStages;
-    uint64_t* tm_full = empty + kMaxStages;
-    uint64_t* tm_empty = tm_full + kBufs;
-    uint64_t* sc_full = tm_empty + kBufs;
-    uint64_t* sc_empty = sc_full + kScaleSlots;
-    uint64_t* done = sc_empty + kScaleSlots;
-    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(done + 1);
-    uint32_t* s_failed = s_tmem + 1;  // a wait of this CTA ran out; one of the cluster did
-    uint32_t* s_run = s_tmem + 4;     // splits: where a run of 4 columns is summed up (cluster address)
+    // everything in shared memory by 32-bit address
+    const uint32_t ring = (smem_addr(smem_raw) + 1023) & ~1023u;
+    const uint32_t stage_bytes = (uint32_t)(a.x_rows + kWRows) * kBK;
+    const uint32_t staging = ring + a.stages * stage_bytes;
+    const uint32_t scales = staging + a.staging_bytes;
+    const uint32_t full = scales + kScaleSlots * kScaleBatch * kScaleWords * 4;
+    const uint32_t empty = full + kMaxStages * 8;
+    const uint32_t tm_full = empty + kMaxStages * 8;
+    const uint32_t tm_empty = tm_full + kMaxBufs * 8;
+    const uint32_t sc_full = tm_empty + kMaxBufs * 8;
+    const uint32_t sc_empty = sc_full + kScaleSlots * 8;
+    const uint32_t done = sc_empty + kScaleSlots * 8;
+    const uint32_t words = done + 8;
+    uint8_t* generic = smem_raw + (words - smem_addr(smem_raw));
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(generic);
+    volatile uint32_t* s_failed = s_tmem + 1;  // a wait of this CTA ran out; one of the cluster did
+    uint32_t* s_run = s_tmem + 4;              // splits: where a run of 4 columns is summed up (cluster address)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int splits = PAIR ? 1 : a.splits;
+    // splits have few groups, and with half of the TMEM the next launch's CTA
+    // can allocate its own while this one runs
+    const int bufs = PAIR || splits > 1 ? 2 : 4;
+    const uint32_t tmem_cols = bufs * BN;
     const int cluster = PAIR ? 2 : splits;
     const int rank = cluster > 1 ? (int)cluster_rank() : 0;
     const int first = blockIdx.x / cluster, step = gridDim.x / cluster;
@@ -335,22 +388,22 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
         prefetch_tensormap(&xmap);
         prefetch_tensormap(&wmap);
         for (int i = 0; i < a.stages; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
+            bar_init(full + i * 8, 1);
+            bar_init(empty + i * 8, 1);
         }
-        for (int i = 0; i < kBufs; ++i) {
-            mbar_init(&tm_full[i], 1);
-            mbar_init(&tm_empty[i], (PAIR ? 2 : 1) * kSumWarps);
+        for (int i = 0; i < bufs; ++i) {
+            bar_init(tm_full + i * 8, 1);
+            bar_init(tm_empty + i * 8, (PAIR ? 2 : 1) * kSumWarps);
         }
         for (int i = 0; i < kScaleSlots; ++i) {
-            mbar_init(&sc_full[i], 2);
-            mbar_init(&sc_empty[i], kSumWarps);
+            bar_init(sc_full + i * 8, 2);
+            bar_init(sc_empty + i * 8, kSumWarps);
         }
-        mbar_init(done, 1);
+        bar_init(done, 1);
         fence_barrier_init();
         s_failed[0] = s_failed[1] = 0;
     }
-    if (warp == kSumWarps + 1) tmem_alloc<PAIR>(s_tmem, TMEM_COLS);
+    if (warp == kSumWarps + 1) tmem_alloc<PAIR>(words, tmem_cols);
     if (!PAIR && splits > 1 && warp == kSumWarps + 2) {
         // run r of 32 belongs to split r * splits / 32; its sums lie at
         // [run][split][row] there, 16 bytes of padding per run
@@ -380,21 +433,15 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
             for (int t = first; t < tiles && ok; t += step) {
                 const int m0 = tile_m(t), w0 = tile_n(t) + (PAIR ? rank * kWRows : 0);
                 for (int g = g0; g < g1; ++g) {
-                    ok = mbar_wait_warp(&empty[r.slot], r.phase ^ 1);
+                    const uint32_t bar = full + r.slot * 8, st = ring + r.slot * stage_bytes;
+                    ok = bar_wait(empty + r.slot * 8, r.phase ^ 1);
                     if (!ok) break;
-                    uint8_t* st = smem + r.slot * stage_bytes;
                     if (elect_one()) {
-                        if constexpr (PAIR) {
-                            // the first CTA's barrier counts both CTAs' bytes
-                            const uint32_t bar = cluster_addr(&full[r.slot], 0);
-                            if (rank == 0) mbar_arrive_expect_tx(&full[r.slot], 2 * (uint32_t)stage_bytes);
-                            tma_load_2d_pair(st, &xmap, bar, g * kBK, m0);
-                            tma_load_2d_pair(st + a.x_rows * kBK, &wmap, bar, g * kBK, w0);
-                        } else {
-                            mbar_arrive_expect_tx(&full[r.slot], (uint32_t)stage_bytes);
-                            tma_load_2d(st, &xmap, &full[r.slot], g * kBK, m0);
-                            tma_load_2d(st + a.x_rows * kBK, &wmap, &full[r.slot], g * kBK, w0);
-                        }
+                        // (a pair: the first CTA's barrier counts both CTAs' bytes)
+                        const uint32_t at = PAIR ? cluster_addr(bar, 0) : bar;
+                        if (!PAIR || rank == 0) bar_expect(bar, (PAIR ? 2 : 1) * stage_bytes);
+                        tma_load<PAIR>(st, &xmap, at, g * kBK, m0);
+                        tma_load<PAIR>(st + a.x_rows * kBK, &wmap, at, g * kBK, w0);
                     }
                     __syncwarp();
                     ++issued;
@@ -412,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
                         q.phase ^= 1;
                     }
                     --q.slot;
-                    (void)mbar_wait_warp(&full[q.slot], q.phase);
+                    (void)bar_wait(full + q.slot * 8, q.phase);
                 }
                 if (lane == 0) s_failed[0] = 1;
             }
@@ -420,30 +467,34 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
             // ---- MMA issue -----------------------------------------------
             constexpr uint32_t idesc = f8_idesc<(PAIR ? 2 : 1) * kBM, BN>();
             Ring r, b;
+            const uint64_t xdesc = sw128_kmajor_desc(ring);
+            const uint64_t wdesc = sw128_kmajor_desc(ring + a.x_rows * kBK);
             for (int t = first; t < tiles && ok; t += step) {
                 for (int g = g0; g < g1; ++g) {
-                    ok = mbar_wait_warp(&tm_empty[b.slot], b.phase ^ 1) && mbar_wait_warp(&full[r.slot], r.phase);
+                    // (descriptors count 16 bytes; the sums' release comes
+                    // last and is what the multiplies usually wait for)
+                    const uint32_t off = r.slot * (stage_bytes / 16);
+                    const uint64_t ad = xdesc + off, bd = wdesc + off;
+                    const uint32_t d = tmem + (uint32_t)(b.slot * BN);
+                    ok = bar_wait(full + r.slot * 8, r.phase) && bar_wait(tm_empty + b.slot * 8, b.phase ^ 1);
                     if (!ok) break;
                     tc_after();
-                    const uint32_t xa = smem_addr(smem) + r.slot * stage_bytes, wa = xa + a.x_rows * kBK;
-                    const uint64_t ad = sw128_kmajor_desc(xa), bd = sw128_kmajor_desc(wa);
                     if (elect_one()) {
 #pragma unroll
-                        for (int kk = 0; kk < kBK / 32; ++kk)  // (32 bytes further: 2 in units of 16)
-                            mma_f8<PAIR>(tmem + (uint32_t)(b.slot * BN), ad + 2 * kk, bd + 2 * kk, idesc, (uint32_t)kk);
-                        mma_commit<PAIR>(&empty[r.slot]);
-                        mma_commit<PAIR>(&tm_full[b.slot]);
+                        for (int kk = 0; kk < kBK / 32; ++kk) mma_f8<PAIR>(d, ad + 2 * kk, bd + 2 * kk, idesc, (uint32_t)kk);
+                        mma_commit<PAIR>(tm_full + b.slot * 8);
+                        mma_commit<PAIR>(empty + r.slot * 8);
                     }
                     __syncwarp();
                     r.next(a.stages);
-                    b.next(kBufs);
+                    b.next(bufs);
                 }
             }
             if (!ok) {
                 // every multiply issued so far ends before the memory is given back
                 if (elect_one()) mma_commit<PAIR>(done);
                 __syncwarp();
-                (void)mbar_wait_warp(done, 0);
+                (void)bar_wait(done, 0);
                 if (lane == 0) s_failed[0] = 1;
             }
         } else if (warp >= kSumWarps + 2) {
@@ -465,17 +516,17 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
                         v1[j] = live1 && g < g1 ? xs[(size_t)g * a.M + 32] : 0.f;
                         w[j] = live_w && g < g1 ? ws[g] : 0.f;
                     }
-                    ok = mbar_wait_warp(&sc_empty[r.slot], r.phase ^ 1);
+                    ok = bar_wait(sc_empty + r.slot * 8, r.phase ^ 1);
                     if (!ok) break;
 #pragma unroll
                     for (int j = 0; j < kScaleBatch; ++j) {
-                        float* dst = scales + (r.slot * kScaleBatch + j) * kScaleWords;
-                        dst[part * 64 + lane] = v0[j];
-                        dst[part * 64 + lane + 32] = v1[j];
-                        if (part == 0 && lane < BN / 128) dst[kBM + lane] = w[j];
+                        const uint32_t dst = scales + ((r.slot * kScaleBatch + j) * kScaleWords + lane) * 4;
+                        st_shared_f(dst + part * 256, v0[j]);
+                        st_shared_f(dst + part * 256 + 128, v1[j]);
+                        if (part == 0 && lane < BN / 128) st_shared_f(dst + kBM * 4, w[j]);
                     }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&sc_full[r.slot]);
+                    if (lane == 0) bar_arrive(sc_full + r.slot * 8);
                     r.next(kScaleSlots);
                 }
             }
@@ -488,7 +539,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
         // ---- sums ----------------------------------------------------------
         const int quad = warp & 3, half = warp >> 2;
         const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * HALF);
-        uint8_t* stg = reinterpret_cast<uint8_t*>(staging) + warp * kWarpStaging<PAIR>;
+        // a buffer's release goes to the CTA that issues the multiplies
+        const uint32_t tm_free = PAIR ? cluster_addr(tm_empty, 0) : tm_empty;
+        const uint32_t stg = staging + warp * kWarpStaging;
         if (!PAIR && cluster > 1) cluster_wait();
         Ring b, r;
         for (int t = first; t < tiles && ok; t += step) {
@@ -497,43 +550,57 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
             float2 acc[HALF / 2];
 #pragma unroll
             for (int c = 0; c < HALF / 2; ++c) acc[c] = make_float2(0.f, 0.f);
-            for (int g = g0; g < g1; ++g) {
-                const int j = (g - g0) % kScaleBatch;
-                if (j == 0) ok = mbar_wait_warp(&sc_full[r.slot], r.phase);
-                ok = ok && mbar_wait_warp(&tm_full[b.slot], b.phase);
+            for (int gb = g0; gb < g1; gb += kScaleBatch) {
+                ok = bar_wait(sc_full + r.slot * 8, r.phase);
                 if (!ok) break;
-                tc_after();
-                const float* sc = scales + (r.slot * kScaleBatch + j) * kScaleWords;
-                const float s = sc[quad * 32 + lane] * sc[kBM + (BN > 128 ? half : 0)];
-                if (rows_live) {
-                    // the next 32 columns are on their way while these are added
-                    // (a load takes about 75 cycles whatever its width: with
-                    // 16 columns at a time a group took 600)
-                    const float2 s2 = make_float2(s, s);
-                    uint32_t v[2][32];
+                // (the weight's scale is the same word for the whole warp)
+                float sg[kScaleBatch];
+                {
+                    const uint32_t sc = scales + r.slot * (kScaleBatch * kScaleWords * 4);
+#pragma unroll
+                    for (int j = 0; j < kScaleBatch; ++j)
+                        sg[j] = ld_shared_f(sc + (j * kScaleWords + quad * 32 + lane) * 4) *
+                                ld_shared_f(sc + (j * kScaleWords + kBM + (BN > 128 ? half : 0)) * 4);
+                    __syncwarp();
+                    if (lane == 0) mbar_release<false>(sc_empty + r.slot * 8);
+                    r.next(kScaleSlots);
+                }
+#pragma unroll
+                for (int j = 0; j < kScaleBatch; ++j) {
+                    if (gb + j >= g1) break;
                     const uint32_t at = taddr + (uint32_t)(b.slot * BN);
-                    tmem_ld32(at, v[0]);
+                    const uint32_t freed = tm_free + b.slot * 8;
+                    ok = bar_wait(tm_full + b.slot * 8, b.phase);
+                    if (!ok) break;
+                    b.next(bufs);
+                    tc_after();
+                    if (rows_live) {
+                        // the next 32 columns are on their way while these are
+                        // added (a load takes about 75 cycles whatever its
+                        // width); the buffer is free once the last ones are here
+                        const float2 s2 = make_float2(sg[j], sg[j]);
+                        uint32_t v[2][32];
+                        tmem_ld32(at, v[0]);
 #pragma unroll
-                    for (int i = 0; i < HALF / 32; ++i) {
-                        tmem_wait_ld(v[i & 1]);
-                        if (i + 1 < HALF / 32) tmem_ld32(at + (uint32_t)(i + 1) * 32, v[(i + 1) & 1]);
+                        for (int i = 0; i < HALF / 32; ++i) {
+                            tmem_wait_ld(v[i & 1]);
+                            if (i + 1 < HALF / 32) {
+                                tmem_ld32(at + (uint32_t)(i + 1) * 32, v[(i + 1) & 1]);
+                            } else {
+                                tc_before();
+                                if (lane == 0) mbar_release<PAIR>(freed);
+                            }
 #pragma unroll
-                        for (int c = 0; c < 16; ++c)
-                            acc[i * 16 + c] = ffma2(
-                                make_float2(__uint_as_float(v[i & 1][2 * c]), __uint_as_float(v[i & 1][2 * c + 1])), s2,
-                                acc[i * 16 + c]);
+                            for (int c = 0; c < 16; ++c)
+                                acc[i * 16 + c] = ffma2(
+                                    make_float2(__uint_as_float(v[i & 1][2 * c]), __uint_as_float(v[i & 1][2 * c + 1])),
+                                    s2, acc[i * 16 + c]);
+                        }
+                    } else if (lane == 0) {
+                        mbar_release<PAIR>(freed);
                     }
                 }
-                tc_before();
-                __syncwarp();
-                const bool last = j == kScaleBatch - 1 || g + 1 == g1;
-                if (lane == 0) {
-                    if (PAIR && rank) mbar_arrive_cluster(cluster_addr(&tm_empty[b.slot], 0));
-                    else mbar_arrive(&tm_empty[b.slot]);
-                    if (last) mbar_arrive(&sc_empty[r.slot]);
-                }
-                b.next(kBufs);
-                if (last) r.next(kScaleSlots);
+                if (!ok) break;
             }
             if (!ok) break;
             if (!PAIR && splits > 1) {
@@ -546,12 +613,12 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
                         st_cluster_f4(s_run[(half * HALF + c) / 4] + mine,
                                       make_float4(acc[c / 2].x, acc[c / 2].y, acc[c / 2 + 1].x, acc[c / 2 + 1].y));
                 }
-            } else if (PAIR && a.tma_out) {
+            } else if (a.tma_out) {
                 // 128 bytes of each of the warp's rows at a time, swizzled as
                 // the tensor map has it, stored by TMA (which drops what lies
                 // past the last row or column)
                 if (rows_live) {
-                    const uint32_t row = smem_addr(stg) + lane * 128;
+                    const uint32_t row = stg + lane * 128;
                     const uint32_t swz = lane & 7;
                     if (a.out_dtype == COTTUS_F32) {
 #pragma unroll
@@ -566,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
                             }
                             fence_proxy_async_smem();
                             __syncwarp();
-                            if (lane == 0 && nh + c0 < a.N) tma_store_2d(&omap, stg, (nh + c0) * 4, m0);
+                            if (lane == 0 && nh + c0 < a.N) tma_store(&omap, stg, (nh + c0) * 4, m0);
                         }
                     } else {
                         const bool f16 = a.out_dtype == COTTUS_F16;
@@ -586,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
                             }
                             fence_proxy_async_smem();
                             __syncwarp();
-                            if (lane == 0 && nh + c0 < a.N) tma_store_2d(&omap, stg, (nh + c0) * 2, m0);
+                            if (lane == 0 && nh + c0 < a.N) tma_store(&omap, stg, (nh + c0) * 2, m0);
                         }
                     }
                 }
@@ -597,28 +664,28 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
                 for (int c0 = 0; c0 < HALF; c0 += 16) {
                     __syncwarp();
 #pragma unroll
-                    for (int c = 0; c < 16; c += 4)
-                        *reinterpret_cast<float4*>(reinterpret_cast<float*>(stg) + lane * kStagePitch + c) =
-                            make_float4(acc[(c0 + c) / 2].x, acc[(c0 + c) / 2].y, acc[(c0 + c) / 2 + 1].x,
-                                        acc[(c0 + c) / 2 + 1].y);
+                    for (int c = 0; c < 16; c += 4) {
+                        const float2 u = acc[(c0 + c) / 2], w = acc[(c0 + c) / 2 + 1];
+                        st_shared_u4(stg + (lane * kStagePitch + c) * 4, make_uint4(__float_as_uint(u.x), __float_as_uint(u.y),
+                                                                                   __float_as_uint(w.x), __float_as_uint(w.y)));
+                    }
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int rr = i * 8 + (lane >> 2), n = nh + c0 + (lane & 3) * 4;
-                        const float4 v =
-                            *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(stg) + rr * kStagePitch + (lane & 3) * 4);
+                        const float4 v = ld_shared_f4(stg + (rr * kStagePitch + (lane & 3) * 4) * 4);
                         if (m0 + rr < a.M && n < a.N) store_out4(a, m0 + rr, n, v);
                     }
                 }
             }
         }
-        if (PAIR && lane == 0) tma_store_done();
+        if (lane == 0) tma_store_done();
         if (!ok && lane == 0) s_failed[0] = 1;
     }
     __syncwarp();
     if (!PAIR && splits > 1) {
         __syncthreads();
-        if (threadIdx.x < splits && s_failed[0]) st_cluster_u32(cluster_addr(s_failed + 1, threadIdx.x), 1u);
+        if (threadIdx.x < splits && s_failed[0]) st_cluster_u32(cluster_addr(words + 8, threadIdx.x), 1u);
         __syncwarp();
         cluster_arrive();
         cluster_wait();  // every CTA's partial sums are where they are added
@@ -629,11 +696,11 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
             const int sh = runs > 16 ? 5 : (runs > 8 ? 4 : (runs > 4 ? 3 : 2));  // lanes per row
             const int run = threadIdx.x & ((1 << sh) - 1), n = n0 + (run0 + run) * 4;
             if (run < runs && n < a.N) {
-                const float4* p = reinterpret_cast<const float4*>(staging) + run * (splits * a.x_rows + 1);
+                const uint32_t p = staging + run * (splits * a.x_rows + 1) * 16;
                 for (int row = threadIdx.x >> sh; row < rows; row += kThreads >> sh) {
-                    float4 v = p[row];
+                    float4 v = ld_shared_f4(p + row * 16);
                     for (int q = 1; q < splits; ++q) {
-                        const float4 w = p[q * a.x_rows + row];
+                        const float4 w = ld_shared_f4(p + (q * a.x_rows + row) * 16);
                         v.x += w.x;
                         v.y += w.y;
                         v.z += w.z;
@@ -651,7 +718,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
         cluster_wait();
     }
     if (threadIdx.x == 0 && s_failed[0]) report(a.status, COTTUS_STATUS_TIMEOUT);
-    if (warp == kSumWarps + 1) tmem_free<PAIR>(tmem, TMEM_COLS);
+    if (warp == kSumWarps + 1) tmem_free<PAIR>(tmem, tmem_cols);
 }
 
 int fail(int code, const std::string& msg) { return set_error(code, msg); }
@@ -713,7 +780,7 @@ template <int BN, bool PAIR>
 cudaError_t launch_linear(const cottus_fp8_linear_params* p, LinArgs a, int grid, cudaStream_t st) {
     cudaError_t err = cudaSuccess;
     a.x_rows = p->rows < kBM ? (p->rows + 7) / 8 * 8 : kBM;
-    a.staging_bytes = kSumWarps * kWarpStaging<PAIR>;
+    a.staging_bytes = kSumWarps * kWarpStaging;
     if (a.splits > 1) a.staging_bytes = (32 + a.splits - 1) / a.splits * (a.splits * a.x_rows + 1) * 16;
     const size_t stage = (size_t)(a.x_rows + kWRows) * kBK;
     const size_t rest = 1024 + (size_t)a.staging_bytes + kTailBytes;
@@ -730,7 +797,7 @@ cudaError_t launch_linear(const cottus_fp8_linear_params* p, LinArgs a, int grid
     if (err != cudaSuccess) return err;
     CUtensorMap omap = wmap;  // (not read without tma_out)
     const int es = dtype_bytes(p->out_dtype);
-    a.tma_out = PAIR && !p->residual && aligned(p->out, 16) && (size_t)p->out_features * es % 16 == 0;
+    a.tma_out = a.splits == 1 && !p->residual && aligned(p->out, 16) && (size_t)p->out_features * es % 16 == 0;
     if (a.tma_out) {
         omap = make_tensor_map_2d_u8(p->out, (uint64_t)p->out_features * es, p->rows, (uint64_t)p->out_features * es, 128, 32,
                                      true, &err);
