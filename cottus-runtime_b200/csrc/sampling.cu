@@ -10,7 +10,8 @@
 //
 // A row belongs to one thread-block cluster; each CTA holds a contiguous
 // slice of it in shared memory and the row is read from HBM once.
-//   1. smallest key (= the maximum, at its lowest index);
+//   1. the maximum, while the slice is loaded (greedy rows then look for its
+//      first place and are done);
 //   2. with top-k or top-p: a histogram (count, mass) of the distance to the
 //      maximum, 128 bins per octave, merged over the cluster; the bin in
 //      which the count or the mass passes its target; its few members are
@@ -20,10 +21,16 @@
 //   3. the kept mass per warp, each warp owning a contiguous run of indices,
 //      then the one warp whose run holds uniform * mass walks it.
 //
-// Weights: exp in fp64, held as 64-bit fixed point (47 - 43 fractional bits,
-// so that a row's sum fits).  Integer sums do not depend on their order, so
-// atomics leave no trace in the result, and a border is missed only where the
-// draw falls within 2^-45 or so of it.
+// Weights are 64-bit fixed point (43 to 47 fractional bits, so that a row's sum
+// fits): integer sums do not depend on their order, so atomics leave no trace
+// in the result.  exp is table-driven (P. Tang, ACM Trans. Math. Softw. 15,
+// 1989): with y = (logit - max) log2(e) / T in two fp32 words and
+// y = k + j / 256 + r, |r| <= 2^-9,  2^y = 2^k 2^(j/256) (1 + q(r)), the table
+// exact to fixed point and the cubic q < 2^-9 in one fp32 word, so a weight is
+// off by 2^-32 of itself.  (A vocabulary of 2^17 near-equal tokens then draws
+// another token than exact arithmetic once in some 10^6 rows.)  exp in fp64
+// took twice the time of everything else together; it serves the settings
+// that fp32 words cannot hold (temperatures beyond 1e-6 or 1e6, infinities).
 //
 // Bounds: HBM for many rows; at one row the chain of cluster barriers (about
 // nine with all filters).
@@ -66,10 +73,15 @@ struct SampleArgs {
     int vocab, slice, raw_bytes, frac_bits;
 };
 
+constexpr int kDirect = 1024;  // largest top_k that one CTA finishes from the list
+constexpr int kTable = 256;    // 2^(j/256)
+
 // Shared memory behind the slice.
 struct Shared {
+    u64 exp2_table[kTable];  // with one bit more than the weights
+    uint32_t count[kBins];  // histogram: members,
     union {
-        uint32_t hist[4][kBins];  // count and three 16-bit limbs of the mass
+        uint32_t limb[3][kBins];  // and their mass in limbs of 16 bits
         u64 list[kList];
     };
     uint32_t mcnt[kBins];  // merged over the cluster
@@ -146,18 +158,53 @@ __device__ __forceinline__ float from_desc(uint32_t d) {
 __device__ __forceinline__ bool candidate(float x) { return x > -INFINITY; }  // false for -inf and NaN
 __device__ __forceinline__ u64 order_key(float x, uint32_t index) { return ((u64)desc_bits(x) << 32) | index; }
 
-// The weight of a logit: exp in fp64, 0 where fixed point cannot hold it.
+// The weight of a logit, in units of 2^-frac.
 struct Weight {
     float top;
-    double inv_t, unit, least;
-    __device__ __forceinline__ double z(float x) const { return ((double)x - (double)top) * inv_t; }
-    __device__ __forceinline__ double operator()(float x) const {
-        if (x == top) return 1.0;
-        if (top == INFINITY) return 0.0;
-        const double v = z(x);
-        return v < least ? 0.0 : exp(v);
+    double inv_t;
+    int frac;
+    bool plain;       // fp32 words hold the exponent
+    float c, cl;      // log2(e) / T in two words
+    const u64* table;
+
+    __device__ __forceinline__ void set(float max, float temperature, int frac_bits, const u64* exp2_table) {
+        top = max;
+        inv_t = 1.0 / (double)temperature;
+        frac = frac_bits;
+        const double cd = 1.4426950408889634 * inv_t;
+        c = (float)cd;
+        cl = (float)(cd - (double)c);
+        plain = cd > 1e-6 && cd < 1e6 && fabsf(max) < 1e30f;
+        table = exp2_table;
     }
-    __device__ __forceinline__ u64 fixed(double w) const { return __double2ull_rn(w * unit); }
+    __device__ __forceinline__ double unit() const { return (double)(1ull << frac); }
+    __device__ __forceinline__ double z(float x) const { return x == top ? 0.0 : ((double)x - (double)top) * inv_t; }
+    __device__ __noinline__ u64 general(float x) const {
+        if (x == top) return 1ull << frac;
+        if (top == INFINITY || !candidate(x)) return 0;
+        const double v = z(x);
+        return v < -(frac + 2) * 0.6931471805599453 ? 0 : __double2ull_rn(exp(v) * unit());
+    }
+    __device__ __forceinline__ u64 operator()(float x) const { return plain ? fast(x) : general(x); }
+    // (0 for -inf and NaN)
+    __device__ __forceinline__ u64 fast(float x) const {
+        // x - top = d + e exactly
+        const float d = x - top, b = d - x, e = (x - (d - b)) - (top + b);
+        const float y = d * c;
+        const float yl = fmaf(e, c, fmaf(d, cl, fmaf(d, c, -y)));
+        // m = rint(256 y): the low bits of y 256 + 1.5 2^23
+        const float magic = 12582912.f;
+        const float t = fmaf(y, 256.f, magic);
+        const int m = __float_as_int(t) - __float_as_int(magic);
+        const float r = fmaf(t - magic, -1.f / 256.f, y) + yl;
+        // 2^r - 1 = sum (r ln 2)^i / i!
+        const float q = r * fmaf(r, fmaf(r, 0.0555041087f, 0.240226507f), 0.693147181f);
+        const int qi = __float_as_int(fmaf(q, 2147483648.f, magic)) - __float_as_int(magic);
+        const u64 p = table[m & (kTable - 1)];
+        const u64 v = p + (u64)(((long long)(int)(p >> 18) * qi) >> 13);  // p < 2^49
+        const int sh = -(m >> 8) & 63;
+        return y > -(float)(frac + 2) ? ((v >> sh) + 1) >> 1 : 0;
+    }
 };
 
 // Level-one bin: monotone in the distance to the maximum.
@@ -169,26 +216,44 @@ __device__ __forceinline__ int distance_bin(float top, float x) {
 
 template <typename XT>
 struct Row {
-    const SampleArgs& a;
+    static constexpr int E = 16 / (int)sizeof(XT);  // logits per 16-byte vector
     Shared& s;
-    const XT* x;    // the slice in shared memory
-    int lo, n;      // its first index and length
-    int rank, size; // of this CTA in the cluster
+    const uint4* vec;  // the slice in shared memory, -inf before and behind it
+    int lo, n;         // index of the first vector's first element; vectors
+    int rank, size;    // of this CTA in the cluster
     Weight weight;
 
-    __device__ __forceinline__ float at(int i) const { return to_f32(x[i]); }
+    __device__ __forceinline__ static void unpack(const uint4& u, float (&v)[E]) {
+        const XT* x = reinterpret_cast<const XT*>(&u);
+#pragma unroll
+        for (int k = 0; k < E; ++k) v[k] = to_f32(x[k]);
+    }
+    // f(logit, index) for every candidate of the slice
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        for (int j = threadIdx.x; j < n; j += kT) {
+            float v[E];
+            unpack(vec[j], v);
+#pragma unroll
+            for (int k = 0; k < E; ++k)
+                if (candidate(v[k])) f(v[k], lo + j * E + k);
+        }
+    }
 
     __device__ void clear_hist() const {
-        for (int i = threadIdx.x; i < 4 * kBins; i += kT) s.hist[0][i] = 0;
+        for (int i = threadIdx.x; i < kBins; i += kT) {
+            s.count[i] = 0;
+            s.limb[0][i] = s.limb[1][i] = s.limb[2][i] = 0;
+        }
         __syncthreads();
     }
     __device__ __forceinline__ void add(int bin, float v, bool mass) const {
-        atomicAdd(&s.hist[0][bin], 1u);
+        atomicAdd(&s.count[bin], 1u);
         if (mass) {
-            const u64 w = weight.fixed(weight(v));
-            if (w & 0xFFFF) atomicAdd(&s.hist[1][bin], (uint32_t)(w & 0xFFFF));
-            if ((w >> 16) & 0xFFFF) atomicAdd(&s.hist[2][bin], (uint32_t)((w >> 16) & 0xFFFF));
-            if (w >> 32) atomicAdd(&s.hist[3][bin], (uint32_t)(w >> 32));
+            const u64 w = weight(v);
+            if (w & 0xFFFF) atomicAdd(&s.limb[0][bin], (uint32_t)(w & 0xFFFF));
+            if ((w >> 16) & 0xFFFF) atomicAdd(&s.limb[1][bin], (uint32_t)((w >> 16) & 0xFFFF));
+            if (w >> 32) atomicAdd(&s.limb[2][bin], (uint32_t)(w >> 32));
         }
     }
     // Merges the cluster's histograms into every CTA's mcnt / mmass.
@@ -200,9 +265,9 @@ struct Row {
             uint32_t c = 0;
             u64 m = 0;
             for (int q = 0; q < size; ++q) {
-                c += ld_cluster(mapa(&s.hist[0][b], q));
-                m += (u64)ld_cluster(mapa(&s.hist[1][b], q)) + ((u64)ld_cluster(mapa(&s.hist[2][b], q)) << 16) +
-                     ((u64)ld_cluster(mapa(&s.hist[3][b], q)) << 32);
+                c += ld_cluster(mapa(&s.count[b], q));
+                m += (u64)ld_cluster(mapa(&s.limb[0][b], q)) + ((u64)ld_cluster(mapa(&s.limb[1][b], q)) << 16) +
+                     ((u64)ld_cluster(mapa(&s.limb[2][b], q)) << 32);
             }
             for (int q = 0; q < size; ++q) {
                 st_cluster(mapa(&s.mcnt[b], q), c);
@@ -284,10 +349,7 @@ struct Row {
     // Level one: the histogram of the distance to the maximum.
     __device__ void build_l1(bool mass) const {
         clear_hist();
-        for (int i = threadIdx.x; i < n; i += kT) {
-            const float v = at(i);
-            if (candidate(v)) add(distance_bin(weight.top, v), v, mass);
-        }
+        each([&](float v, int) { add(distance_bin(weight.top, v), v, mass); });
         merge_hist();
     }
     // The mass of all candidates, from the level-one histogram.
@@ -301,6 +363,116 @@ struct Row {
         for (int w = 0; w < kW; ++w) m += s.wsum[w];
         __syncthreads();
         return m;
+    }
+
+    // Sorts the first m entries of this CTA's list, ascending.
+    __device__ void sort_list(int m) const {
+        int pow2 = 2;
+        while (pow2 < m) pow2 <<= 1;
+        for (int i = m + threadIdx.x; i < pow2; i += kT) s.list[i] = kNoKey;
+        __syncthreads();
+        for (int w = 2; w <= pow2; w <<= 1)
+            for (int j = w >> 1; j; j >>= 1) {
+                for (int i = threadIdx.x; i < pow2 / 2; i += kT) {
+                    const int p0 = ((i & ~(j - 1)) << 1) | (i & (j - 1)), p1 = p0 | j;
+                    const u64 u = s.list[p0], v = s.list[p1];
+                    if ((u > v) == ((p0 & w) == 0)) {
+                        s.list[p0] = v;
+                        s.list[p1] = u;
+                    }
+                }
+                __syncthreads();
+            }
+    }
+    // Sum of `own` over the threads before this one; `total` over all.
+    __device__ u64 block_before(u64 own, u64& total) const {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        const u64 incl = warp_scan(own, lane);
+        __syncthreads();  // (earlier readers of wsum are done)
+        if (lane == 31) s.wsum[warp] = incl;
+        __syncthreads();
+        u64 before = incl - own;
+        total = 0;
+        for (int w = 0; w < kW; ++w) {
+            if (w < warp) before += s.wsum[w];
+            total += s.wsum[w];
+        }
+        return before;
+    }
+    // Smallest value of the block's threads, in every thread.
+    __device__ uint32_t block_min(uint32_t v) const {
+        __syncthreads();
+        if (threadIdx.x == 0) s.pick_bin = 0xFFFFFFFFu;
+        __syncthreads();
+        v = __reduce_min_sync(0xffffffffu, v);
+        if ((threadIdx.x & 31) == 0) atomicMin(&s.pick_bin, v);
+        __syncthreads();
+        return s.pick_bin;
+    }
+
+    // The whole choice among the m <= kList keys of this CTA's list, which
+    // hold the row's first top_k candidates: filters, then the draw.
+    __device__ void solve_row(int m, int top_k, float top_p, float min_p, float u, int32_t* token, float* logprob) const {
+        sort_list(m);
+        if (m > top_k) m = top_k;
+        constexpr int PER = kList / kT;
+        const int at = threadIdx.x * PER;
+        u64 w[PER], own = 0, total;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            w[j] = at + j < m ? weight(from_desc((uint32_t)(s.list[at + j] >> 32))) : 0;
+            own += w[j];
+        }
+        u64 run = block_before(own, total);
+        // entries that stay: up to the one at which the mass reaches its
+        // share, and with at least the least weight; both cut the order off
+        const double t = top_p < 1.f ? (double)top_p * (double)total : (double)total;
+        const u64 least = min_p > 0.f ? __double2ull_ru((double)min_p * weight.unit()) : 0;
+        uint32_t cut = (uint32_t)m;
+#pragma unroll
+        for (int j = PER - 1; j >= 0; --j) {
+            u64 incl = run;
+            for (int i = 0; i <= j; ++i) incl += w[i];
+            if (at + j < m) {
+                if (top_p < 1.f && (double)incl >= t) cut = at + j + 1;
+                if (w[j] < least) cut = at + j;
+            }
+        }
+        const int kept = (int)block_min(cut);
+        // the draw, in index order: (index, logit) keys, sorted
+        u64 again[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const u64 key = at + j < kept ? s.list[at + j] : kNoKey;
+            again[j] = (key << 32) | (key >> 32);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (at + j < kept) s.list[at + j] = again[j];
+        __syncthreads();
+        sort_list(kept);
+        own = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            w[j] = at + j < kept ? weight(from_desc((uint32_t)s.list[at + j])) : 0;
+            own += w[j];
+        }
+        run = block_before(own, total);
+        const double draw = (double)u * (double)total;
+        if ((double)(run + own) > draw && !((double)run > draw)) {
+            bool found = false;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                run += w[j];
+                if (!found && (double)run > draw) {
+                    found = true;
+                    *token = (int32_t)(s.list[at + j] >> 32);
+                    if (logprob)
+                        *logprob = (float)(weight.z(from_desc((uint32_t)s.list[at + j])) - log((double)total / weight.unit()));
+                }
+            }
+        }
     }
 
     // The threshold key at which the running count reaches k, or the running
@@ -327,25 +499,21 @@ struct Row {
         while (p.in_cnt > (uint32_t)kList) {
             // split the bin: its members' key range in kBins equal parts
             u64 mn = kNoKey, mx = 0;
-            for (int i = threadIdx.x; i < n; i += kT) {
-                const float v = at(i);
-                if (!candidate(v)) continue;
-                const u64 key = order_key(v, (uint32_t)(lo + i));
-                if (!member(v, key)) continue;
+            each([&](float v, int i) {
+                const u64 key = order_key(v, (uint32_t)i);
+                if (!member(v, key)) return;
                 mn = key < mn ? key : mn;
                 mx = key > mx ? key : mx;
-            }
+            });
             mn = cluster_min(mn);
             mx = ~cluster_min(~mx);
             int sh = 0;
             while (((mx - mn) >> sh) >= (u64)kBins) ++sh;
             clear_hist();
-            for (int i = threadIdx.x; i < n; i += kT) {
-                const float v = at(i);
-                if (!candidate(v)) continue;
-                const u64 key = order_key(v, (uint32_t)(lo + i));
+            each([&](float v, int i) {
+                const u64 key = order_key(v, (uint32_t)i);
                 if (member(v, key)) add((int)((key - mn) >> sh), v, need_mass);
-            }
+            });
             merge_hist();
             l1 = false;
             p = pick_bin(by_mass, k - before_cnt, before_mass, t);
@@ -360,41 +528,18 @@ struct Row {
         if (threadIdx.x == 0) s.list_n = 0;
         csync();  // (also: nobody reads a histogram any more, the list may take its place)
         {
-            const int lane = threadIdx.x & 31;
             const uint32_t counter = mapa(&s.list_n, 0), list0 = mapa(&s.list[0], 0);
-            for (int i0 = threadIdx.x - lane; i0 < n; i0 += kT) {
-                const int i = i0 + lane;
-                const float v = i < n ? at(i) : -INFINITY;
-                const u64 key = order_key(v, (uint32_t)(lo + i));
-                const bool in = candidate(v) && member(v, key);
-                const uint32_t mask = __ballot_sync(0xffffffffu, in);
-                if (!mask) continue;
-                uint32_t at0 = 0;
-                if (lane == 0) at0 = atom_add_cluster(counter, __popc(mask));
-                at0 = __shfl_sync(0xffffffffu, at0, 0);
-                const uint32_t pos = at0 + __popc(mask & ((1u << lane) - 1));
-                if (in && pos < (uint32_t)kList) st_cluster(list0 + pos * 8, key);
-            }
+            each([&](float v, int i) {
+                const u64 key = order_key(v, (uint32_t)i);
+                if (!member(v, key)) return;
+                const uint32_t pos = atom_add_cluster(counter, 1);
+                if (pos < (uint32_t)kList) st_cluster(list0 + pos * 8, key);
+            });
         }
         csync();
         if (rank == 0) {
             const int m = (int)(s.list_n < (uint32_t)kList ? s.list_n : (uint32_t)kList);
-            int pow2 = 2;
-            while (pow2 < m) pow2 <<= 1;
-            for (int i = m + threadIdx.x; i < pow2; i += kT) s.list[i] = kNoKey;
-            __syncthreads();
-            for (int w = 2; w <= pow2; w <<= 1)
-                for (int j = w >> 1; j; j >>= 1) {
-                    for (int i = threadIdx.x; i < pow2 / 2; i += kT) {
-                        const int p0 = ((i & ~(j - 1)) << 1) | (i & (j - 1)), p1 = p0 | j;
-                        const u64 u = s.list[p0], v = s.list[p1];
-                        if ((u > v) == ((p0 & w) == 0)) {
-                            s.list[p0] = v;
-                            s.list[p1] = u;
-                        }
-                    }
-                    __syncthreads();
-                }
+            sort_list(m);
             // prefix masses of the sorted members, in runs of `per` per thread
             const int per = (m + kT - 1) / kT;
             const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -402,7 +547,7 @@ struct Row {
             if (need_mass)
                 for (int j = 0; j < per; ++j) {
                     const int i = threadIdx.x * per + j;
-                    if (i < m) own += weight.fixed(weight(from_desc((uint32_t)(s.list[i] >> 32))));
+                    if (i < m) own += weight(from_desc((uint32_t)(s.list[i] >> 32)));
                 }
             const u64 incl = warp_scan(own, lane);
             if (lane == 31) s.wsum[warp] = incl;
@@ -414,7 +559,7 @@ struct Row {
             for (int j = 0; j < per; ++j) {
                 const int i = threadIdx.x * per + j;
                 if (i >= m) break;
-                if (need_mass) run += weight.fixed(weight(from_desc((uint32_t)(s.list[i] >> 32))));
+                if (need_mass) run += weight(from_desc((uint32_t)(s.list[i] >> 32)));
                 const bool hit = i == m - 1 || (by_mass ? (double)run >= t : before_cnt + (uint32_t)i + 1 >= k);
                 if (hit) {
                     atomicMin(&s.pick_bin, (uint32_t)i);
@@ -432,7 +577,7 @@ struct Row {
                 u64 r = run0;
                 if (need_mass)
                     for (int i = threadIdx.x * per; i <= hit; ++i)
-                        r += weight.fixed(weight(from_desc((uint32_t)(s.list[i] >> 32))));
+                        r += weight(from_desc((uint32_t)(s.list[i] >> 32)));
                 const u64 key = s.list[hit];
                 for (int q = 0; q < size; ++q) {
                     st_cluster(mapa(&s.res[0], q), key);
@@ -466,7 +611,7 @@ struct Row {
 };
 
 template <typename XT>
-__global__ void __launch_bounds__(kT) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kT, 2) sample_kernel(const SampleArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     Shared& s = *reinterpret_cast<Shared*>(smem + a.raw_bytes);
     uint32_t rank_u, size_u;
@@ -474,64 +619,108 @@ __global__ void __launch_bounds__(kT) sample_kernel(const SampleArgs a) {
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size_u));
     const int rank = (int)rank_u, size = (int)size_u;
     const int row = blockIdx.x / size;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int lo = rank * a.slice < a.vocab ? rank * a.slice : a.vocab;
-    const int n = a.vocab - lo < a.slice ? a.vocab - lo : a.slice;
-    const XT* g = reinterpret_cast<const XT*>(a.logits) + (size_t)row * a.vocab + lo;
-    const int mis = (int)(reinterpret_cast<uintptr_t>(g) & 15);
-    XT* x = reinterpret_cast<XT*>(smem + mis);
+    const int lane = threadIdx.x & 31;
+    // this CTA's logits [i0, i1), in whole 16-byte vectors from the boundary
+    // at or before the first one
+    constexpr int E = Row<XT>::E;
+    const int i0 = rank * a.slice < a.vocab ? rank * a.slice : a.vocab;
+    const int i1 = a.vocab - i0 < a.slice ? a.vocab : i0 + a.slice;
+    const XT* g = reinterpret_cast<const XT*>(a.logits) + (size_t)row * a.vocab + i0;
+    const int pad = (int)(reinterpret_cast<uintptr_t>(g) & 15) / (int)sizeof(XT);
+    const int vecs = i1 > i0 ? (pad + i1 - i0 + E - 1) / E : 0;
+    uint4* vec = reinterpret_cast<uint4*>(smem);
     carrive();  // (awaited below: no CTA's shared memory is written before it has started)
+    for (int i = threadIdx.x; i < kBins; i += kT) s.count[i] = 0;
+    if (threadIdx.x == 0) s.list_n = 0;
+    if (threadIdx.x < kTable) {
+        const double unit = (double)(1ull << (a.frac_bits + 1));
+        s.exp2_table[threadIdx.x] = __double2ull_rn(exp2(threadIdx.x * (1.0 / kTable)) * unit);
+    }
     grid_dependency_wait();
     grid_dependents_launch();
-    // the slice, at the same offset from a 16-byte boundary as in memory:
-    // whole 16-byte runs, and single elements at its two ends
+    float top = -INFINITY;  // (fmaxf passes NaN over)
     {
-        constexpr int E = 16 / (int)sizeof(XT);
-        const int head = mis ? ((16 - mis) / (int)sizeof(XT) < n ? (16 - mis) / (int)sizeof(XT) : n) : 0;
-        const int runs = (n - head) / E;
-        const uint4* src = reinterpret_cast<const uint4*>(g + head);
-        uint4* dst = reinterpret_cast<uint4*>(x + head);
+        const uint4* src = reinterpret_cast<const uint4*>(g - pad);
+        const int whole0 = pad ? 1 : 0, whole1 = (pad + i1 - i0) / E;  // vectors that lie within the row
 #pragma unroll 4
-        for (int i = threadIdx.x; i < runs; i += kT) dst[i] = ld_once(src + i);
-        if (threadIdx.x < head) x[threadIdx.x] = g[threadIdx.x];
-        const int tail = head + runs * E;
-        if (threadIdx.x < n - tail) x[tail + threadIdx.x] = g[tail + threadIdx.x];
+        for (int j = whole0 + threadIdx.x; j < whole1; j += kT) {
+            const uint4 u = ld_once(src + j);
+            vec[j] = u;
+            float v[E];
+            Row<XT>::unpack(u, v);
+#pragma unroll
+            for (int k = 0; k < E; ++k) top = fmaxf(top, v[k]);
+        }
+        // the first and the last vector, where they reach past the row
+        if (threadIdx.x < 2 * E) {
+            const int j = threadIdx.x < E ? 0 : vecs - 1, k = threadIdx.x % E, i = j * E + k - pad;
+            if (vecs > 0 && (j < whole0 || j >= whole1)) {
+                const bool in = i >= 0 && i < i1 - i0;
+                const XT v = in ? g[i] : from_float<XT>(-INFINITY);
+                reinterpret_cast<XT*>(vec)[j * E + k] = v;
+                if (in) top = fmaxf(top, to_f32(v));
+            }
+        }
     }
     float temp = a.temperature ? a.temperature[row] : 1.f;
     const float u_in = a.uniforms[row];
-    int top_k = a.top_k ? a.top_k[row] : 0;
+    const int top_k = a.top_k ? a.top_k[row] : 0;
     const float top_p = a.top_p ? a.top_p[row] : 1.f;
     const float min_p = a.min_p ? a.min_p[row] : 0.f;
     cwait();
-    __syncthreads();
 
-    Row<XT> r{a, s, x, lo, n, rank, size, {}};
-    u64 front = kNoKey;
-    for (int i = threadIdx.x; i < n; i += kT) {
-        const float v = r.at(i);
-        if (candidate(v)) {
-            const u64 key = order_key(v, (uint32_t)(lo + i));
-            front = key < front ? key : front;
-        }
-    }
-    front = r.cluster_min(front);
-    if (front == kNoKey || !(temp > 0.f)) {  // nothing to choose from, or greedy
+    Row<XT> r{s, vec, i0 - pad, vecs, rank, size, {}};
+    const u64 best = r.cluster_min((u64)desc_bits(top));
+    top = from_desc((uint32_t)best);
+    const bool none = !(top > -INFINITY);
+    if (none || !(temp > 0.f) || top_k == 1 || top_p <= 0.f || min_p > 1.f) {
+        // nothing to choose from, or the front candidate alone
+        u64 first = kNoKey;
+        if (!none) r.each([&](float v, int i) { first = v == top && (u64)i < first ? (u64)i : first; });
+        first = r.cluster_min(first);
         if (rank == 0 && threadIdx.x == 0) {
-            const bool none = front == kNoKey;
-            a.tokens[row] = none ? -1 : (int32_t)(uint32_t)front;
+            a.tokens[row] = none ? -1 : (int32_t)first;
             if (a.logprobs) a.logprobs[row] = none ? -INFINITY : 0.f;
             if (none) report(a.status, COTTUS_STATUS_NO_TOKEN);
         }
         return;
     }
-    r.weight.top = from_desc((uint32_t)(front >> 32));
-    r.weight.inv_t = 1.0 / (double)temp;
-    r.weight.unit = (double)(1ull << a.frac_bits);
-    r.weight.least = -(a.frac_bits + 2) * 0.6931471805599453;
+    r.weight.set(top, temp, a.frac_bits, s.exp2_table);
 
     u64 thr = kNoKey;
     const bool by_p = top_p < 1.f;  // (false for NaN)
     const bool by_k = top_k > 0 && top_k < a.vocab;
+    // uniform in [0, 1): 1 - 2^-24 is the largest fp32 below 1 (NaN counts as 0)
+    const float u = u_in > 0.f ? fminf(u_in, 0.99999994f) : 0.f;
+    if (by_k && top_k <= kDirect) {
+        // few candidates: their histogram by count alone, every CTA adding up
+        // the cluster's; the first CTA gets all up to the bin in which the
+        // count reaches top_k, and does the rest by itself
+        r.each([&](float v, int) { atomicAdd(&s.count[distance_bin(top, v)], 1u); });
+        csync();
+        for (int b = threadIdx.x; b < kBins; b += kT) {
+            uint32_t c = 0;
+            for (int q = 0; q < size; ++q) c += ld_cluster(mapa(&s.count[b], q));
+            s.mcnt[b] = c;
+            s.mmass[b] = 0;
+        }
+        __syncthreads();
+        const auto p = r.pick_bin(false, (uint32_t)top_k, 0, 0.0);
+        if (p.before_cnt + p.in_cnt <= (uint32_t)kList) {  // (no bin picked: top_k candidates or fewer)
+            const uint32_t counter = mapa(&s.list_n, 0), list0 = mapa(&s.list[0], 0);
+            r.each([&](float v, int i) {
+                if (distance_bin(top, v) > p.bin) return;
+                const uint32_t pos = atom_add_cluster(counter, 1);
+                if (pos < (uint32_t)kList) st_cluster(list0 + pos * 8, order_key(v, (uint32_t)i));
+            });
+            csync();
+            if (rank == 0)
+                r.solve_row((int)(s.list_n < (uint32_t)kList ? s.list_n : (uint32_t)kList), top_k, top_p, min_p, u,
+                            a.tokens + row, a.logprobs ? a.logprobs + row : nullptr);
+            return;
+        }
+        csync();  // (the histogram is about to be cleared)
+    }
     bool l1 = false;
     if (by_k) {
         u64 mass = 0;
@@ -548,62 +737,71 @@ __global__ void __launch_bounds__(kT) sample_kernel(const SampleArgs a) {
         thr = r.select(true, 0, (double)top_p * (double)mass, kNoKey, true, l1, mass);
     }
 
-    // the kept mass: each warp owns a contiguous run of indices
-    const int run = (n + kT - 1) / kT * 32;
-    const int w0 = warp * run, w1 = w0 + run < n ? w0 + run : n;
-    const double least_w = min_p > 0.f ? (double)min_p : 0.0;  // (0 for NaN)
-    auto kept = [&](int i) -> u64 {
-        const float v = r.at(i);
-        if (!candidate(v)) return 0;
-        const u64 key = order_key(v, (uint32_t)(lo + i));
-        if (key > thr) return 0;
-        const double w = r.weight(v);
-        return w >= least_w || key == front ? r.weight.fixed(w) : 0;
+    // the kept mass: each thread owns a contiguous run of vectors (an odd
+    // number, so that the lanes of a warp read from different banks)
+    const int run = (vecs + kT - 1) / kT | 1;
+    const int v0 = threadIdx.x * run < vecs ? threadIdx.x * run : vecs, v1 = v0 + run < vecs ? v0 + run : vecs;
+    // min-p in the weights' units (0: off, as for NaN; the largest weight, 1, always stays)
+    const u64 least_w = min_p > 0.f ? __double2ull_ru((double)min_p * r.weight.unit()) : 0;
+    const bool filtered = thr != kNoKey || least_w > 0 || !r.weight.plain;
+    auto kept = [&](float v, int i) -> u64 {
+        if (!candidate(v) || order_key(v, (uint32_t)i) > thr) return 0;
+        const u64 w = r.weight(v);
+        return w >= least_w ? w : 0;
     };
     u64 own = 0;
-    for (int i = w0 + lane; i < w1; i += 32) own += kept(i);
-    own = warp_sum(own);
-    if (lane == 0) s.wsum[warp] = own;
-    __syncthreads();
-    u64 cta = 0;
-    for (int w = 0; w < kW; ++w) cta += s.wsum[w];
+    if (!filtered) {
+        for (int j = v0; j < v1; ++j) {
+            float v[E];
+            Row<XT>::unpack(vec[j], v);
+#pragma unroll
+            for (int k = 0; k < E; ++k) own += r.weight.fast(v[k]);
+        }
+    } else {
+        for (int j = v0; j < v1; ++j) {
+            float v[E];
+            Row<XT>::unpack(vec[j], v);
+#pragma unroll
+            for (int k = 0; k < E; ++k) own += kept(v[k], r.lo + j * E + k);
+        }
+    }
+    u64 cta;
+    u64 base = r.block_before(own, cta);
     if (threadIdx.x < size) st_cluster(mapa(&s.slot[1][rank], threadIdx.x), cta);
     csync();
-    u64 base = 0, total = 0;
+    u64 total = 0;
     for (int q = 0; q < size; ++q) {
         if (q < rank) base += s.slot[1][q];
         total += s.slot[1][q];
     }
-    for (int w = 0; w < warp; ++w) base += s.wsum[w];
-    // uniform in [0, 1): 1 - 2^-24 is the largest fp32 below 1 (NaN counts as 0)
-    const float u = u_in > 0.f ? fminf(u_in, 0.99999994f) : 0.f;
     const double t = (double)u * (double)total;
-    // the warp in whose run the running sum first exceeds t
-    if ((double)(base + own) > t && !((double)base > t)) {
-        u64 before = base;
-        for (int i0 = w0; i0 < w1; i0 += 32) {
+    // the thread in whose run the running sum first exceeds t; its warp
+    // walks the run, a logit per lane
+    const uint32_t owner = __ballot_sync(0xffffffffu, (double)(base + own) > t && !((double)base > t));
+    if (owner) {
+        const int who = __ffs(owner) - 1;
+        u64 before = __shfl_sync(0xffffffffu, base, who);
+        const int e0 = __shfl_sync(0xffffffffu, v0, who) * E, e1 = __shfl_sync(0xffffffffu, v1, who) * E;
+        for (int i0 = e0; i0 < e1; i0 += 32) {
             const int i = i0 + lane;
-            const u64 m = i < w1 ? kept(i) : 0;
-            const u64 sum = before + warp_scan(m, lane);
-            const uint32_t hit = __ballot_sync(0xffffffffu, (double)sum > t);
+            const float v = i < e1 ? to_f32(reinterpret_cast<const XT*>(vec)[i]) : -INFINITY;
+            const u64 m = filtered ? kept(v, r.lo + i) : r.weight.fast(v);
+            const u64 incl = before + warp_scan(m, lane);
+            const uint32_t hit = __ballot_sync(0xffffffffu, (double)incl > t);
             if (hit) {
                 if (lane == __ffs(hit) - 1) {
-                    a.tokens[row] = lo + i;
-                    if (a.logprobs) {
-                        const float v = r.at(i);
-                        const double z = v == r.weight.top ? 0.0 : r.weight.z(v);
-                        a.logprobs[row] = (float)(z - log((double)total / r.weight.unit));
-                    }
+                    a.tokens[row] = r.lo + i;
+                    if (a.logprobs) a.logprobs[row] = (float)(r.weight.z(v) - log((double)total / r.weight.unit()));
                 }
                 break;
             }
-            before = __shfl_sync(0xffffffffu, sum, 31);
+            before = __shfl_sync(0xffffffffu, incl, 31);
         }
     }
 }
 
 // Dynamic shared memory of a CTA that holds `slice` logits.
-size_t sample_smem(int slice, int es) { return ((size_t)slice * es + 31) / 16 * 16 + sizeof(Shared); }
+size_t sample_smem(int slice, int es) { return ((size_t)slice * es + 46) / 16 * 16 + sizeof(Shared); }
 
 template <typename XT>
 cudaError_t launch_sample(SampleArgs a, int batch, int cluster, cudaStream_t st) {
