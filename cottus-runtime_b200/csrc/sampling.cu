@@ -74,24 +74,23 @@ struct SampleArgs {
 };
 
 constexpr int kDirect = 1024;  // largest top_k that one CTA finishes from the list
+constexpr int kCountSort = 192;  // entries up to which a list is sorted by counting
 constexpr int kTable = 256;    // 2^(j/256)
 
 // Shared memory behind the slice.
 struct Shared {
     u64 exp2_table[kTable];  // with one bit more than the weights
     uint32_t count[kBins];  // histogram: members,
-    union {
-        uint32_t limb[3][kBins];  // and their mass in limbs of 16 bits
-        u64 list[kList];
-    };
+    uint32_t limb[3][kBins];  // and their mass in limbs of limb_bits
+    u64 list[kList];
     uint32_t mcnt[kBins];  // merged over the cluster
     u64 mmass[kBins];
     u64 wsum[kW];
     uint32_t wcnt[kW];
-    u64 slot[2][kMaxCluster];  // one word from each CTA
+    u64 slot[3][kMaxCluster];  // one word from each CTA
     u64 res[4];                // broadcast by the first CTA
     u64 pick_mass;
-    uint32_t pick_cnt, pick_bin, list_n;
+    uint32_t pick_cnt, pick_in, pick_bin, list_n;
 };
 
 __device__ __forceinline__ void carrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -116,10 +115,20 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t a) {
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
     return v;
 }
+__device__ __forceinline__ uint4 ld_cluster_u4(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
 __device__ __forceinline__ uint32_t atom_add_cluster(uint32_t a, uint32_t v) {
     uint32_t r;
     asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(r) : "r"(a), "r"(v) : "memory");
     return r;
+}
+__device__ __forceinline__ u64 ld_cluster_u64(uint32_t a) {
+    u64 v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+    return v;
 }
 
 __device__ __forceinline__ u64 shfl_xor(u64 v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
@@ -214,6 +223,14 @@ __device__ __forceinline__ int distance_bin(float top, float x) {
     return b < 0 ? 0 : (b < kBins ? b : kBins - 1);
 }
 
+// The bin's distances: at least near_edge, below far_edge (comparisons of
+// the distance alone, for passes over all logits).
+__device__ __forceinline__ float near_edge(int bin) { return bin <= 0 ? -INFINITY : __uint_as_float((uint32_t)(bin + (125 << 7)) << 16); }
+__device__ __forceinline__ float far_edge(int bin) {
+    return bin >= kBins - 1 ? INFINITY : __uint_as_float((uint32_t)(bin + 1 + (125 << 7)) << 16);
+}
+__device__ __forceinline__ float distance(float top, float x) { return x == top ? 0.f : top - x; }
+
 template <typename XT>
 struct Row {
     static constexpr int E = 16 / (int)sizeof(XT);  // logits per 16-byte vector
@@ -221,6 +238,7 @@ struct Row {
     const uint4* vec;  // the slice in shared memory, -inf before and behind it
     int lo, n;         // index of the first vector's first element; vectors
     int rank, size;    // of this CTA in the cluster
+    int limb_bits;     // a slice's limbs add up within 32 bits
     Weight weight;
 
     __device__ __forceinline__ static void unpack(const uint4& u, float (&v)[E]) {
@@ -251,30 +269,49 @@ struct Row {
         atomicAdd(&s.count[bin], 1u);
         if (mass) {
             const u64 w = weight(v);
-            if (w & 0xFFFF) atomicAdd(&s.limb[0][bin], (uint32_t)(w & 0xFFFF));
-            if ((w >> 16) & 0xFFFF) atomicAdd(&s.limb[1][bin], (uint32_t)((w >> 16) & 0xFFFF));
-            if (w >> 32) atomicAdd(&s.limb[2][bin], (uint32_t)(w >> 32));
+            const uint32_t mask = (1u << limb_bits) - 1;
+            atomicAdd(&s.limb[0][bin], (uint32_t)w & mask);
+            atomicAdd(&s.limb[1][bin], (uint32_t)(w >> limb_bits) & mask);
+            const uint32_t high = (uint32_t)(w >> (2 * limb_bits));
+            if (high) atomicAdd(&s.limb[2][bin], high);  // (the likeliest few)
         }
     }
-    // Merges the cluster's histograms into every CTA's mcnt / mmass.
+    // Adds the cluster's histograms up, every CTA for itself, into its mcnt /
+    // mmass (16 loads of four bins per thread, all in flight).  The
+    // histogram may be cleared, or its words used, after the next cluster barrier.
     __device__ void merge_hist() const {
         csync();
-        const int per = kBins / size;
-        for (int i = threadIdx.x; i < per; i += kT) {
-            const int b = rank * per + i;
-            uint32_t c = 0;
-            u64 m = 0;
-            for (int q = 0; q < size; ++q) {
-                c += ld_cluster(mapa(&s.count[b], q));
-                m += (u64)ld_cluster(mapa(&s.limb[0][b], q)) + ((u64)ld_cluster(mapa(&s.limb[1][b], q)) << 16) +
-                     ((u64)ld_cluster(mapa(&s.limb[2][b], q)) << 32);
-            }
-            for (int q = 0; q < size; ++q) {
-                st_cluster(mapa(&s.mcnt[b], q), c);
-                st_cluster(mapa(&s.mmass[b], q), m);
+        constexpr int Q = kBins / 4;  // runs of four bins
+        static_assert(2 * Q == kT, "half of the threads add counts and low limbs, half the others");
+        const int b = (threadIdx.x % Q) * 4;
+        const bool low = threadIdx.x < Q;
+        const uint32_t* a0 = low ? &s.count[b] : &s.limb[1][b];
+        const uint32_t* a1 = low ? &s.limb[0][b] : &s.limb[2][b];
+        uint4 x[kMaxCluster], y[kMaxCluster];
+#pragma unroll
+        for (int q = 0; q < kMaxCluster; ++q) {
+            x[q] = q < size ? ld_cluster_u4(mapa(a0, q)) : make_uint4(0, 0, 0, 0);
+            y[q] = q < size ? ld_cluster_u4(mapa(a1, q)) : make_uint4(0, 0, 0, 0);
+        }
+        u64 cx[4] = {0, 0, 0, 0}, cy[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int q = 0; q < kMaxCluster; ++q) {
+            cx[0] += x[q].x, cx[1] += x[q].y, cx[2] += x[q].z, cx[3] += x[q].w;
+            cy[0] += y[q].x, cy[1] += y[q].y, cy[2] += y[q].z, cy[3] += y[q].w;
+        }
+        if (low) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s.mcnt[b + j] = (uint32_t)cx[j];
+                s.mmass[b + j] = cy[j];
             }
         }
-        csync();
+        __syncthreads();
+        if (!low) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s.mmass[b + j] += (cx[j] << limb_bits) + (cy[j] << (2 * limb_bits));
+        }
+        __syncthreads();
     }
 
     struct Pick {
@@ -285,65 +322,55 @@ struct Row {
     // The bin in which the running count reaches k (by_mass false) or the
     // running mass, on top of mass0, reaches t.
     __device__ Pick pick_bin(bool by_mass, uint32_t k, u64 mass0, double t) const {
+        return pick_bin(by_mass, k, mass0, t, [&](int b) { return s.mcnt[b]; }, [&](int b) { return s.mmass[b]; });
+    }
+    template <typename FC, typename FM>
+    __device__ __forceinline__ Pick pick_bin(bool by_mass, uint32_t k, u64 mass0, double t, FC cnt_of, FM mass_of) const {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         constexpr int PER = kBins / kT;
-        uint32_t c = 0;
-        u64 m = 0;
+        uint32_t c[PER], ctot = 0;
+        u64 m[PER], mtot = 0;
+#pragma unroll
         for (int j = 0; j < PER; ++j) {
-            c += s.mcnt[threadIdx.x * PER + j];
-            m += s.mmass[threadIdx.x * PER + j];
+            ctot += c[j] = cnt_of(threadIdx.x * PER + j);
+            mtot += m[j] = mass_of(threadIdx.x * PER + j);
         }
-        const uint32_t ci = warp_scan(c, lane);
-        const u64 mi = warp_scan(m, lane);
+        uint32_t cb = warp_scan(ctot, lane);
+        u64 mb = warp_scan(mtot, lane);
+        __syncthreads();  // (earlier readers of these words are done)
         if (lane == 31) {
-            s.wcnt[warp] = ci;
-            s.wsum[warp] = mi;
+            s.wcnt[warp] = cb;
+            s.wsum[warp] = mb;
         }
-        if (threadIdx.x == 0) s.pick_bin = kBins;
+        if (threadIdx.x == 0) {
+            s.pick_bin = kBins;
+            s.pick_cnt = s.pick_in = 0;
+            s.pick_mass = 0;
+        }
         __syncthreads();
-        uint32_t cb = ci - c;
-        u64 mb = mi - m;
-        for (int w = 0; w < warp; ++w) {
-            cb += s.wcnt[w];
-            mb += s.wsum[w];
-        }
+        cb -= ctot;
+        mb += mass0 - mtot;
+#pragma unroll
+        for (int w = 0; w < kW; ++w)
+            if (w < warp) {
+                cb += s.wcnt[w];
+                mb += s.wsum[w];
+            }
+#pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const int b = threadIdx.x * PER + j;
-            const uint32_t cc = s.mcnt[b];
-            const u64 mm = s.mmass[b];
-            const bool before = by_mass ? (double)(mass0 + mb) < t || (mass0 + mb == 0) : cb < k;
-            const bool reached = by_mass ? (double)(mass0 + mb + mm) >= t : cb + cc >= k;
-            // the first bin that reaches the target from below is the pick
-            // (empty bins before it reach nothing new)
-            if (cc && before && reached) atomicMin(&s.pick_bin, (uint32_t)b);
-            cb += cc;
-            mb += mm;
+            // sums only grow, so one bin takes them past the target
+            const bool here = by_mass ? (double)mb < t && (double)(mb + m[j]) >= t : cb < k && cb + c[j] >= k;
+            if (here) {
+                s.pick_bin = threadIdx.x * PER + j;
+                s.pick_cnt = cb;
+                s.pick_in = c[j];
+                s.pick_mass = mb - mass0;
+            }
+            cb += c[j];
+            mb += m[j];
         }
         __syncthreads();
-        const int bin = (int)s.pick_bin;
-        // sums before the picked bin, by its owner
-        if (bin < kBins && threadIdx.x == bin / PER) {
-            uint32_t c2 = ci - c;
-            u64 m2 = mi - m;
-            for (int w = 0; w < warp; ++w) {
-                c2 += s.wcnt[w];
-                m2 += s.wsum[w];
-            }
-            for (int j = threadIdx.x * PER; j < bin; ++j) {
-                c2 += s.mcnt[j];
-                m2 += s.mmass[j];
-            }
-            s.pick_cnt = c2;
-            s.pick_mass = m2;
-        }
-        __syncthreads();
-        Pick p;
-        p.bin = bin;
-        p.before_cnt = bin < kBins ? s.pick_cnt : 0;
-        p.before_mass = bin < kBins ? s.pick_mass : 0;
-        p.in_cnt = bin < kBins ? s.mcnt[bin] : 0;
-        __syncthreads();
-        return p;
+        return {(int)s.pick_bin, s.pick_cnt, s.pick_in, s.pick_mass};
     }
 
     // Level one: the histogram of the distance to the maximum.
@@ -365,10 +392,50 @@ struct Row {
         return m;
     }
 
-    // Sorts the first m entries of this CTA's list, ascending.
+    // Sorts the first m entries of this CTA's list (all different), ascending.
     __device__ void sort_list(int m) const {
+        if (m <= kCountSort) {
+            // an entry's place is the number of smaller ones, counted by
+            // kT / (m rounded up to a power of two) threads: no barrier until
+            // the end (145 entries: 2k cycles, the bitonic network's 36 steps
+            // 4k; the reads grow with m times the block, so 356 took 18k)
+            int lg = 4;  // log2 of threads per entry, at most 16
+            while (lg > 0 && (m << lg) > kT) --lg;
+            const int e = threadIdx.x >> lg, part = threadIdx.x & ((1 << lg) - 1);
+            const u64 key = e < m ? s.list[e] : kNoKey;
+            uint32_t rank = 0;
+#pragma unroll 4
+            for (int j = part; j < m; j += 1 << lg) rank += s.list[j] < key;
+            for (int o = 1; o < 1 << lg; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+            __syncthreads();
+            if (e < m && part == 0) s.list[rank] = key;
+            __syncthreads();
+            return;
+        }
         int pow2 = 2;
         while (pow2 < m) pow2 <<= 1;
+        if (m <= kT) {
+            // bitonic, an entry per thread; steps within a warp need no barrier
+            u64 key = threadIdx.x < m ? s.list[threadIdx.x] : kNoKey;
+            for (int w = 2; w <= pow2; w <<= 1)
+                for (int j = w >> 1; j; j >>= 1) {
+                    u64 other;
+                    if (j < 32) {
+                        other = shfl_xor(key, j);
+                    } else {
+                        __syncthreads();
+                        s.list[threadIdx.x] = key;
+                        __syncthreads();
+                        other = s.list[threadIdx.x ^ j];
+                    }
+                    const bool small = ((threadIdx.x & j) == 0) == ((threadIdx.x & w) == 0);
+                    key = small == (key < other) ? key : other;
+                }
+            __syncthreads();
+            s.list[threadIdx.x] = key;
+            __syncthreads();
+            return;
+        }
         for (int i = m + threadIdx.x; i < pow2; i += kT) s.list[i] = kNoKey;
         __syncthreads();
         for (int w = 2; w <= pow2; w <<= 1)
@@ -383,6 +450,83 @@ struct Row {
                 }
                 __syncthreads();
             }
+    }
+    // Brings the entries of every CTA's list into this one's, behind its own
+    // (kList in all at most); their number.
+    __device__ int collect_lists() const {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        const uint32_t mine = lane < size ? ld_cluster(mapa(&s.list_n, lane)) : 0;
+        const uint32_t upto = warp_scan(mine, lane);
+        const uint32_t total = __shfl_sync(0xffffffffu, upto, 31);
+        if (warp > 0 && warp < size) {  // (warp q copies CTA q's)
+            const uint32_t m = __shfl_sync(0xffffffffu, mine, warp), at = __shfl_sync(0xffffffffu, upto, warp) - m;
+            const uint32_t from = mapa(&s.list[0], warp);
+#pragma unroll 4
+            for (uint32_t i = lane; i < m; i += 32)
+                if (at + i < (uint32_t)kList) s.list[at + i] = ld_cluster_u64(from + i * 8);
+        }
+        __syncthreads();
+        return (int)(total < (uint32_t)kList ? total : (uint32_t)kList);
+    }
+    // Keeps the entries of this CTA's list of m among which the running count
+    // (from before_cnt) reaches k, or the running mass (from before_mass) t;
+    // their number.  A histogram of the keys, as in select, but of this list
+    // alone (in the words of the merged one, which is lost): sorting 1300
+    // entries took 13k cycles.
+    __device__ int narrow_list(int m, bool by_mass, uint32_t k, double t, uint32_t& before_cnt, u64& before_mass,
+                               bool need_mass) const {
+        constexpr int PER = kList / kT;
+        uint32_t *cnt = s.count, *l0 = s.mcnt, *l1 = reinterpret_cast<uint32_t*>(s.mmass), *l2 = l1 + kBins;
+        u64 key[PER], mn = kNoKey, mx = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int i = threadIdx.x + j * kT;
+            key[j] = i < m ? s.list[i] : kNoKey;
+            if (i < m) {
+                mn = key[j] < mn ? key[j] : mn;
+                mx = key[j] > mx ? key[j] : mx;
+            }
+        }
+        mn = block_min64(mn);
+        mx = ~block_min64(~mx);
+        int sh = 0;
+        while (((mx - mn) >> sh) >= (u64)kBins) ++sh;
+        for (int b = threadIdx.x; b < kBins; b += kT) cnt[b] = l0[b] = l1[b] = l2[b] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (threadIdx.x + j * kT < m) {
+                const int b = (int)((key[j] - mn) >> sh);
+                atomicAdd(&cnt[b], 1u);
+                if (need_mass) {  // (at most 2048 entries: limbs of 16 bits add up within 32)
+                    const u64 w = weight(from_desc((uint32_t)(key[j] >> 32)));
+                    atomicAdd(&l0[b], (uint32_t)w & 0xFFFFu);
+                    atomicAdd(&l1[b], (uint32_t)(w >> 16) & 0xFFFFu);
+                    atomicAdd(&l2[b], (uint32_t)(w >> 32));
+                }
+            }
+        if (threadIdx.x == 0) s.list_n = 0;
+        __syncthreads();
+        const Pick p = pick_bin(by_mass, k - before_cnt, before_mass, t, [&](int b) { return cnt[b]; },
+                                [&](int b) { return (u64)l0[b] + ((u64)l1[b] << 16) + ((u64)l2[b] << 32); });
+        before_cnt += p.before_cnt;
+        before_mass += p.before_mass;
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (threadIdx.x + j * kT < m && (int)((key[j] - mn) >> sh) == p.bin) s.list[atomicAdd(&s.list_n, 1u)] = key[j];
+        __syncthreads();
+        m = (int)s.list_n;
+        __syncthreads();
+        return m;
+    }
+    // Smallest v of the block's threads, in every thread.
+    __device__ u64 block_min64(u64 v) const {
+        v = warp_min(v);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) s.wsum[threadIdx.x >> 5] = v;
+        __syncthreads();
+        for (int w = 0; w < kW; ++w) v = s.wsum[w] < v ? s.wsum[w] : v;
+        return v;
     }
     // Sum of `own` over the threads before this one; `total` over all.
     __device__ u64 block_before(u64 own, u64& total) const {
@@ -416,26 +560,25 @@ struct Row {
         sort_list(m);
         if (m > top_k) m = top_k;
         constexpr int PER = kList / kT;
-        const int at = threadIdx.x * PER;
+        const int per = (m + kT - 1) / kT, at = threadIdx.x * per;  // this thread's run of entries
         u64 w[PER], own = 0, total;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            w[j] = at + j < m ? weight(from_desc((uint32_t)(s.list[at + j] >> 32))) : 0;
+            w[j] = j < per && at + j < m ? weight(from_desc((uint32_t)(s.list[at + j] >> 32))) : 0;
             own += w[j];
         }
         u64 run = block_before(own, total);
         // entries that stay: up to the one at which the mass reaches its
         // share, and with at least the least weight; both cut the order off
-        const double t = top_p < 1.f ? (double)top_p * (double)total : (double)total;
+        const double t = (double)top_p * (double)total;
         const u64 least = min_p > 0.f ? __double2ull_ru((double)min_p * weight.unit()) : 0;
         uint32_t cut = (uint32_t)m;
 #pragma unroll
-        for (int j = PER - 1; j >= 0; --j) {
-            u64 incl = run;
-            for (int i = 0; i <= j; ++i) incl += w[i];
-            if (at + j < m) {
-                if (top_p < 1.f && (double)incl >= t) cut = at + j + 1;
-                if (w[j] < least) cut = at + j;
+        for (int j = 0; j < PER; ++j) {
+            run += w[j];
+            if (j < per && at + j < m) {
+                if (w[j] < least) cut = min(cut, (uint32_t)(at + j));
+                if (top_p < 1.f && (double)run >= t) cut = min(cut, (uint32_t)(at + j + 1));
             }
         }
         const int kept = (int)block_min(cut);
@@ -443,19 +586,19 @@ struct Row {
         u64 again[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const u64 key = at + j < kept ? s.list[at + j] : kNoKey;
+            const u64 key = j < per && at + j < kept ? s.list[at + j] : kNoKey;
             again[j] = (key << 32) | (key >> 32);
         }
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < PER; ++j)
-            if (at + j < kept) s.list[at + j] = again[j];
+            if (j < per && at + j < kept) s.list[at + j] = again[j];
         __syncthreads();
         sort_list(kept);
         own = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            w[j] = at + j < kept ? weight(from_desc((uint32_t)s.list[at + j])) : 0;
+            w[j] = j < per && at + j < kept ? weight(from_desc((uint32_t)s.list[at + j])) : 0;
             own += w[j];
         }
         run = block_before(own, total);
@@ -480,7 +623,7 @@ struct Row {
     // l1: the merged arrays hold the level-one histogram (with masses, where
     // need_mass); false on return if they no longer do.  mass_to (need_mass):
     // the mass of everything up to the threshold.
-    __device__ u64 select(bool by_mass, uint32_t k, double t, u64 limit, bool need_mass, bool& l1, u64& mass_to) const {
+    __device__ __forceinline__ u64 select(bool by_mass, uint32_t k, double t, u64 limit, bool need_mass, bool& l1, u64& mass_to) const {
         if (!l1) build_l1(need_mass);
         l1 = true;
         Pick p = pick_bin(by_mass, k, 0, t);
@@ -505,8 +648,8 @@ struct Row {
                 mn = key < mn ? key : mn;
                 mx = key > mx ? key : mx;
             });
-            mn = cluster_min(mn);
-            mx = ~cluster_min(~mx);
+            mn = cluster_min(mn, 0);
+            mx = ~cluster_min(~mx, 1);
             int sh = 0;
             while (((mx - mn) >> sh) >= (u64)kBins) ++sh;
             clear_hist();
@@ -526,19 +669,18 @@ struct Row {
         }
         // gather the members in the first CTA
         if (threadIdx.x == 0) s.list_n = 0;
-        csync();  // (also: nobody reads a histogram any more, the list may take its place)
-        {
-            const uint32_t counter = mapa(&s.list_n, 0), list0 = mapa(&s.list[0], 0);
-            each([&](float v, int i) {
-                const u64 key = order_key(v, (uint32_t)i);
-                if (!member(v, key)) return;
-                const uint32_t pos = atom_add_cluster(counter, 1);
-                if (pos < (uint32_t)kList) st_cluster(list0 + pos * 8, key);
-            });
-        }
+        __syncthreads();
+        const float d0 = near_edge(level_bin), d1 = far_edge(level_bin);
+        each([&](float v, int i) {
+            const float d = distance(weight.top, v);
+            if (d < d0 || !(d < d1 || d1 == INFINITY)) return;  // not of the picked bin, split up or not
+            const u64 key = order_key(v, (uint32_t)i);
+            if (member(v, key)) s.list[atomicAdd(&s.list_n, 1u)] = key;
+        });
         csync();
         if (rank == 0) {
-            const int m = (int)(s.list_n < (uint32_t)kList ? s.list_n : (uint32_t)kList);
+            int m = collect_lists();
+            while (m > kT) m = narrow_list(m, by_mass, k, t, before_cnt, before_mass, need_mass);
             sort_list(m);
             // prefix masses of the sorted members, in runs of `per` per thread
             const int per = (m + kT - 1) / kT;
@@ -586,26 +728,29 @@ struct Row {
             }
         }
         csync();
+        l1 = false;  // (the first CTA's merged words may have served its list)
         mass_to = s.res[1];
         const u64 thr = s.res[0];
         __syncthreads();
         return thr;
     }
 
-    // Smallest v of the cluster's threads, in every thread.
-    __device__ u64 cluster_min(u64 v) const {
+    // Smallest v of the cluster's threads, in every thread.  `use` names the
+    // words that carry it: not those of the call before, which other CTAs may
+    // still be reading.
+    __device__ u64 cluster_min(u64 v, int use) const {
         v = warp_min(v);
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        __syncthreads();  // (earlier readers of wsum are done)
         if (lane == 0) s.wsum[warp] = v;
         __syncthreads();
         if (warp == 0) {
             v = warp_min(lane < kW ? s.wsum[lane] : kNoKey);
-            if (lane < size) st_cluster(mapa(&s.slot[0][rank], lane), v);
+            if (lane < size) st_cluster(mapa(&s.slot[use][rank], lane), v);
         }
         csync();
         v = kNoKey;
-        for (int q = 0; q < size; ++q) v = s.slot[0][q] < v ? s.slot[0][q] : v;
-        csync();  // the slots may be written again
+        for (int q = 0; q < size; ++q) v = s.slot[use][q] < v ? s.slot[use][q] : v;
         return v;
     }
 };
@@ -669,15 +814,15 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const SampleArgs a) {
     const float min_p = a.min_p ? a.min_p[row] : 0.f;
     cwait();
 
-    Row<XT> r{s, vec, i0 - pad, vecs, rank, size, {}};
-    const u64 best = r.cluster_min((u64)desc_bits(top));
+    Row<XT> r{s, vec, i0 - pad, vecs, rank, size, a.slice <= 32768 ? 17 : 16, {}};
+    const u64 best = r.cluster_min((u64)desc_bits(top), 0);
     top = from_desc((uint32_t)best);
     const bool none = !(top > -INFINITY);
     if (none || !(temp > 0.f) || top_k == 1 || top_p <= 0.f || min_p > 1.f) {
         // nothing to choose from, or the front candidate alone
         u64 first = kNoKey;
         if (!none) r.each([&](float v, int i) { first = v == top && (u64)i < first ? (u64)i : first; });
-        first = r.cluster_min(first);
+        first = r.cluster_min(first, 1);
         if (rank == 0 && threadIdx.x == 0) {
             a.tokens[row] = none ? -1 : (int32_t)first;
             if (a.logprobs) a.logprobs[row] = none ? -INFINITY : 0.f;
@@ -699,42 +844,40 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const SampleArgs a) {
         r.each([&](float v, int) { atomicAdd(&s.count[distance_bin(top, v)], 1u); });
         csync();
         for (int b = threadIdx.x; b < kBins; b += kT) {
-            uint32_t c = 0;
-            for (int q = 0; q < size; ++q) c += ld_cluster(mapa(&s.count[b], q));
-            s.mcnt[b] = c;
+            uint32_t c[kMaxCluster], sum = 0;  // (all loads in flight together)
+#pragma unroll
+            for (int q = 0; q < kMaxCluster; ++q) c[q] = q < size ? ld_cluster(mapa(&s.count[b], q)) : 0;
+#pragma unroll
+            for (int q = 0; q < kMaxCluster; ++q) sum += c[q];
+            s.mcnt[b] = sum;
             s.mmass[b] = 0;
         }
         __syncthreads();
         const auto p = r.pick_bin(false, (uint32_t)top_k, 0, 0.0);
         if (p.before_cnt + p.in_cnt <= (uint32_t)kList) {  // (no bin picked: top_k candidates or fewer)
             const uint32_t counter = mapa(&s.list_n, 0), list0 = mapa(&s.list[0], 0);
+            const float d1 = far_edge(p.bin);
             r.each([&](float v, int i) {
-                if (distance_bin(top, v) > p.bin) return;
-                const uint32_t pos = atom_add_cluster(counter, 1);
-                if (pos < (uint32_t)kList) st_cluster(list0 + pos * 8, order_key(v, (uint32_t)i));
+                const float d = distance(top, v);
+                if (d < d1 || d1 == INFINITY)
+                    st_cluster(list0 + atom_add_cluster(counter, 1) * 8, order_key(v, (uint32_t)i));
             });
             csync();
-            if (rank == 0)
-                r.solve_row((int)(s.list_n < (uint32_t)kList ? s.list_n : (uint32_t)kList), top_k, top_p, min_p, u,
-                            a.tokens + row, a.logprobs ? a.logprobs + row : nullptr);
+            if (rank == 0) r.solve_row((int)s.list_n, top_k, top_p, min_p, u, a.tokens + row, a.logprobs ? a.logprobs + row : nullptr);
             return;
         }
         csync();  // (the histogram is about to be cleared)
     }
+    // first by count, then by mass
     bool l1 = false;
-    if (by_k) {
-        u64 mass = 0;
-        thr = r.select(false, (uint32_t)top_k, 0.0, kNoKey, by_p, l1, mass);
-        if (by_p) {
-            const double t = (double)top_p * (double)mass;
-            thr = r.select(true, 0, t, thr, true, l1, mass);
+    u64 mass = 0;
+    for (int by_mass = by_k ? 0 : 1; by_mass < (by_p ? 2 : 1); ++by_mass) {
+        if (by_mass && !by_k) {  // the whole mass first: one histogram serves both
+            r.build_l1(true);
+            l1 = true;
+            mass = r.l1_mass();
         }
-    } else if (by_p) {
-        // the whole mass first: one histogram serves both
-        r.build_l1(true);
-        l1 = true;
-        u64 mass = r.l1_mass();
-        thr = r.select(true, 0, (double)top_p * (double)mass, kNoKey, true, l1, mass);
+        thr = r.select(by_mass != 0, (uint32_t)top_k, (double)top_p * (double)mass, thr, by_p, l1, mass);
     }
 
     // the kept mass: each thread owns a contiguous run of vectors (an odd
@@ -744,8 +887,10 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const SampleArgs a) {
     // min-p in the weights' units (0: off, as for NaN; the largest weight, 1, always stays)
     const u64 least_w = min_p > 0.f ? __double2ull_ru((double)min_p * r.weight.unit()) : 0;
     const bool filtered = thr != kNoKey || least_w > 0 || !r.weight.plain;
+    const float thr_v = thr == kNoKey ? -INFINITY : from_desc((uint32_t)(thr >> 32));
+    const int thr_i = (int)(uint32_t)thr;
     auto kept = [&](float v, int i) -> u64 {
-        if (!candidate(v) || order_key(v, (uint32_t)i) > thr) return 0;
+        if (!(v > thr_v) && (v != thr_v || i > thr_i)) return 0;  // behind the threshold
         const u64 w = r.weight(v);
         return w >= least_w ? w : 0;
     };
@@ -767,12 +912,12 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const SampleArgs a) {
     }
     u64 cta;
     u64 base = r.block_before(own, cta);
-    if (threadIdx.x < size) st_cluster(mapa(&s.slot[1][rank], threadIdx.x), cta);
+    if (threadIdx.x < size) st_cluster(mapa(&s.slot[2][rank], threadIdx.x), cta);
     csync();
     u64 total = 0;
     for (int q = 0; q < size; ++q) {
-        if (q < rank) base += s.slot[1][q];
-        total += s.slot[1][q];
+        if (q < rank) base += s.slot[2][q];
+        total += s.slot[2][q];
     }
     const double t = (double)u * (double)total;
     // the thread in whose run the running sum first exceeds t; its warp
