@@ -68,6 +68,36 @@ __device__ __forceinline__ void load8_stream(const __nv_bfloat16* p, float (&v)[
     }
 }
 
+// Eight elements in their own type.
+template <typename XT>
+struct Vec8 {
+    union {
+        uint4 u[sizeof(XT) / 2];
+        uint16_t h[8 * sizeof(XT) / 2];
+        uint32_t w[8 * sizeof(XT) / 4];
+    };
+    __device__ __forceinline__ Vec8() {}
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(XT) / 2; ++i) u[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(const XT* p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(XT) / 2; ++i) u[i] = ld_once(reinterpret_cast<const uint4*>(p) + i);
+    }
+    __device__ __forceinline__ void set(int j, XT x) {
+        if constexpr (sizeof(XT) == 4) w[j] = __float_as_uint(to_f32(x));
+        else h[j] = *reinterpret_cast<uint16_t*>(&x);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (sizeof(XT) == 4) v[j] = __uint_as_float(w[j]);
+            else v[j] = to_f32(*reinterpret_cast<const XT*>(&h[j]));
+        }
+    }
+};
+
 // Maximum that keeps a NaN of either side.
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
@@ -94,18 +124,24 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// Eight of them.  The quotients are correctly rounded: q0 = v * RN(1/s) is
-// within an ulp, and q0 + RN(v - q0 s) RN(1/s) is then RN(v / s) (Markstein,
-// IBM J. Res. Dev. 34, 1990), while nothing underflows: v below 2^-10 s is
-// 0 in e4m3 whatever its last bit, and for larger v the remainder stays a
-// normal number where s >= 2^-90.  Smaller, infinite and NaN scales divide.
-// Three packed operations for two quotients instead of two divisions: the
-// 28672 x 8200 bf16 weight took 272 us with divisions.
-__device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float s) {
+// Division by a group's scale.  The quotients are correctly rounded: with
+// r = RN(1/s), q0 = RN(v r) is within an ulp, and q0 + RN(v - q0 s) r is then
+// RN(v / s) (Markstein, IBM J. Res. Dev. 34, 1990) while nothing underflows:
+// v below 2^-10 s is 0 in e4m3 whatever its last bit, and for larger v the
+// remainder stays a normal number where s >= 2^-90.  Smaller, infinite and NaN
+// scales divide.  Three packed operations for two quotients instead of two
+// divisions: the 28672 x 8200 bf16 weight took 272 us with divisions.
+struct Divisor {
+    float s, r;
+    bool plain;
+    __device__ __forceinline__ explicit Divisor(float scale) : s(scale), r(0.f), plain(scale >= 0x1p-90f && scale < INFINITY) {
+        if (plain) r = __frcp_rn(scale);
+    }
+};
+__device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], const Divisor& d) {
     float q[8];
-    if (s >= 0x1p-90f && s < INFINITY) {
-        const float r = __frcp_rn(s);
-        const float2 r2 = make_float2(r, r), ns2 = make_float2(-s, -s);
+    if (d.plain) {
+        const float2 r2 = make_float2(d.r, d.r), ns2 = make_float2(-d.s, -d.s);
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
             const float2 x = make_float2(v[j], v[j + 1]);
@@ -116,7 +152,7 @@ __device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], float s) {
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) q[j] = __fdiv_rn(v[j], s);
+        for (int j = 0; j < 8; ++j) q[j] = __fdiv_rn(v[j], d.s);
     }
     uint2 o;
     o.x = e4m3x2(q[0], q[1]) | (e4m3x2(q[2], q[3]) << 16);

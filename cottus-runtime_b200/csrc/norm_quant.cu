@@ -121,7 +121,7 @@ __global__ void rms_norm_vec_kernel(const NormArgs a) {
         }
         const float s = group_scale(amax16(amax8(h[i])));
         if (live) {
-            *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.out) + e) = e4m3x8(h[i], s);
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.out) + e) = e4m3x8(h[i], Divisor(s));
             if ((v & 15) == 0) a.scales[(size_t)(v >> 4) * a.rows + row] = s;
         }
     }
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
     }
     const float s = group_scale(amax16(amax8(v)));
     if constexpr (VEC) {
-        if (lane * 8 < n) *reinterpret_cast<uint2*>(a.out + base + lane * 8) = e4m3x8(v, s);
+        if (lane * 8 < n) *reinterpret_cast<uint2*>(a.out + base + lane * 8) = e4m3x8(v, Divisor(s));
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -241,10 +241,13 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a) {
     if (live && lane == 0) a.scales[(size_t)g * a.rows + row] = s;
 }
 
-// Blocks: one CTA per 128 x 128 block, 64 elements per thread in registers.
+// Blocks: one CTA per 128 x 128 block, 32 elements per thread, kept as they
+// were loaded (as fp32 they took 64 registers of 256 threads, 2 CTAs per SM and
+// 2.4 TB/s).
 template <typename XT, bool VEC>
-__global__ void __launch_bounds__(256) quant_blocks_kernel(const QuantArgs a) {
-    __shared__ float red[8];
+__global__ void __launch_bounds__(512, sizeof(XT) == 4 ? 2 : 3) quant_blocks_kernel(const QuantArgs a) {
+    __shared__ float red[16];
+    constexpr int R = 4;
     const int cb = blockIdx.x, groups = gridDim.x;
     const long long rb = blockIdx.y;
     const int c0 = cb * 128;
@@ -252,44 +255,49 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(const QuantArgs a) {
     const int lane = threadIdx.x & 15, r0 = threadIdx.x >> 4;
     grid_dependency_wait();
     grid_dependents_launch();
-    float v[8][8];
-    float m = 0.f;
+    Vec8<XT> x[R];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const long long row = rb * 128 + r0 + i * 16;
-        const XT* x = reinterpret_cast<const XT*>(a.x) + (size_t)row * a.cols + c0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    for (int i = 0; i < R; ++i) {
+        const long long row = rb * 128 + r0 + i * 32;
+        const XT* p = reinterpret_cast<const XT*>(a.x) + (size_t)row * a.cols + c0;
+        x[i].clear();
         if (row < a.rows) {
             if constexpr (VEC) {
-                if (lane * 8 < nc) load8_stream(x + lane * 8, v[i]);
+                if (lane * 8 < nc) x[i].load(p + lane * 8);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (lane + j * 16 < nc) v[i][j] = to_f32(x[lane + j * 16]);
+                    if (lane + j * 16 < nc) x[i].set(j, p[lane + j * 16]);
             }
         }
     }
+    float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max_nan(m, amax8(v[i]));
+    for (int i = 0; i < R; ++i) {
+        float v[8];
+        x[i].get(v);
+        m = max_nan(m, amax8(v));
+    }
     m = amax16(m);
     m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 16));
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; ++w) m = max_nan(m, red[w]);
+    m = amax16(red[lane]);
     const float s = group_scale(m);
+    const Divisor d(s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const long long row = rb * 128 + r0 + i * 16;
+    for (int i = 0; i < R; ++i) {
+        const long long row = rb * 128 + r0 + i * 32;
         if (row >= a.rows) continue;
         uint8_t* o = a.out + (size_t)row * a.cols + c0;
+        float v[8];
+        x[i].get(v);
         if constexpr (VEC) {
-            if (lane * 8 < nc) *reinterpret_cast<uint2*>(o + lane * 8) = e4m3x8(v[i], s);
+            if (lane * 8 < nc) *reinterpret_cast<uint2*>(o + lane * 8) = e4m3x8(v, d);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (lane + j * 16 < nc) o[lane + j * 16] = e4m3(v[i][j], s);
+                if (lane + j * 16 < nc) o[lane + j * 16] = e4m3(v[j], s);
         }
     }
     if (threadIdx.x == 0) a.scales[(size_t)rb * groups + cb] = s;
@@ -300,7 +308,7 @@ cudaError_t launch_quant(const QuantArgs& a, bool blocks, cudaStream_t st) {
     const long long groups = (a.cols + 127) / 128;
     if (blocks)
         return launch_pdl(quant_blocks_kernel<XT, VEC>, dim3((unsigned)groups, (unsigned)((a.rows + 127) / 128)),
-                          dim3(256), 0, st, a);
+                          dim3(512), 0, st, a);
     return launch_pdl(quant_rows_kernel<XT, VEC>, dim3((unsigned)((a.rows * groups + 15) / 16)), dim3(256), 0, st, a);
 }
 
