@@ -77,6 +77,7 @@ constexpr int kMaxBufs = 4;     // product buffers in TMEM
 constexpr int kStagePitch = 20; // words per staged row of 16 columns (conflict-free 16-byte accesses)
 constexpr int kScaleSlots = 3;  // of kScaleBatch groups each
 constexpr int kScaleBatch = 4;
+constexpr int kPrefetch = 4;   // groups whose weights are prefetched into L2
 constexpr int kScaleWords = kBM + 4;  // a group's scales: 128 rows, then one per 128 columns of the tile
 constexpr size_t kSmemMax = 232448;   // dynamic shared memory per CTA, 227 KB
 constexpr int kWarpStaging = 32 * 128;  // per sum warp: 128 bytes of each of its rows (or 16 padded columns)
@@ -176,6 +177,12 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[32]) {
                        "+r"(v[i + 6]), "+r"(v[i + 7]));
 }
 
+// The box into L2 (a hint).
+__device__ __forceinline__ void tma_prefetch_l2(const CUtensorMap* map, int c0, int c1) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(c0), "r"(c1)
+                 : "memory");
+}
 // 2-D tiled TMA store from this CTA's shared memory, in the thread's bulk group.
 __device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int c0, int c1) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
@@ -418,6 +425,13 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
     // needs that now, splits before they send their sums)
     if (cluster > 1) cluster_arrive();
     if (PAIR) cluster_wait();
+    // the first groups' weights start on their way to L2 before the preceding
+    // kernel is done (a hint: nothing is read here, and what that kernel still
+    // writes, L2 sees): 64 x 4096 x 4096 8.8 -> 8.6 us in a chain of launches
+    if (warp == kSumWarps && first < tiles && elect_one()) {
+        const int w0 = tile_n(first) + (PAIR ? rank * kWRows : 0);
+        for (int g = g0; g < g1 && g < g0 + kPrefetch; ++g) tma_prefetch_l2(&wmap, g * kBK, w0);
+    }
     grid_dependency_wait();
     // (after the allocation above: a dependent that also allocates TMEM can
     // then only wait for this grid, never the other way round)
@@ -864,8 +878,11 @@ extern "C" int cottus_fp8_linear(const cottus_fp8_linear_params* p, cottus_strea
     const int64_t narrow = (int64_t)((M + 127) / 128) * ((N + 127) / 128), wide = (int64_t)((M + 255) / 256) * ((N + 255) / 256);
     if (narrow >= (int64_t(1) << 30)) return fail(COTTUS_ERR_UNSUPPORTED, "product too large");
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (M > 128 && dev.pairs > 0 && wide >= dev.pairs) {
-        // enough tiles for every SM
+    // The wide tile where the narrow ones do not fit the GPU at once.  K = 4096,
+    // narrow against wide in us: 144 narrow tiles (384 x 6144) 15.4 : 19.4,
+    // 192 (512 x 6144) 25.2 : 19.6, 384 (1024 x 6144) 36.7 : 34.0, 1152 (3000 x
+    // 6144) 90 : 71.  Up to 128 rows half of the wide tile would be empty.
+    if (M > 128 && dev.pairs > 0 && narrow > dev.sms) {
         a.m_tiles = (M + 255) / 256;
         a.n_tiles = (N + 255) / 256;
         a.splits = 1;
