@@ -8,39 +8,39 @@
 //
 // The scales differ from group to group, so a group's 128-deep product is
 // accumulated in tensor memory (four tcgen05.mma of kind::f8f6f4, K = 32
-// each) and then added, scaled, to fp32 sums in registers.  A row of x is a
-// TMEM lane, so a thread's scale is one number for its whole run of columns:
-// one fused multiply-add per element and group.  Per CTA:
+// each) and then added, scaled, to fp32 sums in registers.  Per CTA:
 //
-//   warps 0-7   the sums: warp w reads TMEM lanes 32 (w mod 4) .. + 31,
-//               columns BN/2 (w / 4) .. + BN/2
+//   warps 0-7   the sums: warp w reads TMEM lanes 32 (w mod 4) .. + 31, and
+//               half (w / 4) of the product's columns
 //   warp 8      TMA producer (one thread): ring of stages, one group per stage
 //   warp 9      TMEM allocation and MMA issue (one thread)
-//   warps 10-11 scales: copy each group's row scales and weight scales to a
-//               ring of their own, kScaleBatch groups at once and kScaleSlots
+//   warps 10-11 scales: bring each group's row and weight scales to a ring of
+//               their own, kScaleBatch groups at once and kScaleSlots batches
 //               ahead (read by the sums themselves, one group ahead, a group
 //               took an L2 round trip; so it did with one 4-byte cp.async and
 //               one asynchronous arrival per group)
 //
-// TMEM holds two product buffers, so the tensor cores work on one group while
-// the other is being added up.
+// TMEM holds two to four product buffers, so the tensor cores work on one
+// group while another is being added up.
 //
 // Two tiles:
-//   narrow  128 x 128, one CTA.  A decode batch (rows <= 128) reads the weight
-//           once and is bound by HBM or latency.  Where the weight has fewer
-//           tiles than the GPU has SMs, `splits` CTAs of one cluster share a
-//           tile: each takes a contiguous run of groups and sends its sums to
-//           the CTA that adds them (distributed shared memory, every CTA a
-//           share of the columns), in rank order, so a result does not depend
-//           on timing.  Only the rows that exist are fetched (the TMA box is
-//           as high as the batch, rounded up to 8); the other MMA lanes read
-//           whatever follows in the same stage and are never stored.
+//   narrow  128 rows of the weight (TMEM lanes) by XR = 16, 32, 64 or 128 rows
+//           of x (columns), one CTA.  A decode batch reads the weight once and
+//           is bound by HBM or latency; the multiplies are as many as the
+//           batch needs (with the rows of x as lanes, 128 whatever the batch,
+//           a 37-row product over a 128256-row weight held the GPU at its
+//           power limit, 1.4 GHz).  Where the weight has fewer tiles than the
+//           GPU has SMs, `splits` CTAs of one cluster share a tile: each takes
+//           a contiguous run of groups and sends its sums to the CTA that adds
+//           them (distributed shared memory, every CTA a share of the weight's
+//           rows), in rank order, so a result does not depend on timing.
 //   wide    256 x 256 by a pair of CTAs (cta_group::2): each holds 128 rows of
 //           x and of the weight, and the pair's MMA reads both halves, so an
 //           SM moves 32 KB per 128 x 256 x 128 multiplies.  With the same
 //           128 x 256 per SM as one CTA (48 KB) shared memory was the limit,
 //           reads by the MMA and writes by TMA together: 1270 cycles a group
-//           against the 512 of the multiplies.
+//           against the 512 of the multiplies.  Here a row of x is a lane, and
+//           a thread's scale one number for its 128 columns.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -91,7 +91,7 @@ struct LinArgs {
     const float* residual;
     void* out;
     uint32_t* status;
-    int M, N, groups, n_blocks, m_tiles, n_tiles, splits, stages, x_rows, out_dtype;
+    int M, N, groups, n_blocks, m_tiles, n_tiles, splits, stages, out_dtype;
     int staging_bytes;
     int tma_out;  // whole 128-byte pieces of out may be stored by TMA
     int vec;  // rows of out and residual start on 16 bytes and hold whole runs of 4
@@ -104,7 +104,7 @@ __device__ __forceinline__ uint64_t sw128_kmajor_desc(uint32_t smem_byte_addr) {
 }
 // kind::f8f6f4: e4m3 A and B (format 0), fp32 accumulator, both K-major.
 template <int M, int N>
-constexpr uint32_t f8_idesc() {
+constexpr uint32_t f8_idesc() {  // M lanes, N columns
     return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -154,6 +154,24 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
     else
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+// 8 or 16 columns of this warp's 32 lanes, waited for.
+__device__ __forceinline__ void tmem_get8(uint32_t addr, uint32_t* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_get16(uint32_t addr, uint32_t* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr)
+        : "memory");
 }
 // 32 columns of this warp's 32 lanes.
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
@@ -208,9 +226,8 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t local, uint32_t rank) 
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
     return a;
 }
-__device__ __forceinline__ void st_cluster_f4(uint32_t a, float4 v) {
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
-                 : "memory");
+__device__ __forceinline__ void st_cluster_f(uint32_t a, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
 __device__ __forceinline__ void st_cluster_u32(uint32_t a, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
@@ -335,6 +352,27 @@ __device__ __forceinline__ void store_out4(const LinArgs& a, int m, int n, float
     }
 }
 
+// Sums of weight row n (this thread's) and rows m0 .. of x: a warp stores runs
+// of 32 columns.
+template <int HC>
+__device__ __forceinline__ void store_column(const LinArgs& a, int m0, int n, const float2 (&acc)[HC / 2]) {
+    if (n >= a.N) return;
+    const float* res = a.residual ? a.residual + (size_t)m0 * a.N + n : nullptr;
+    const size_t e = (size_t)m0 * a.N + n;
+    const int rows = a.M - m0;
+    auto each = [&](auto put) {
+#pragma unroll
+        for (int c = 0; c < HC; ++c)
+            if (c < rows) {
+                const float v = c & 1 ? acc[c / 2].y : acc[c / 2].x;
+                put((size_t)c * a.N, res ? v + res[(size_t)c * a.N] : v);
+            }
+    };
+    if (a.out_dtype == COTTUS_F32) each([&](size_t o, float v) { reinterpret_cast<float*>(a.out)[e + o] = v; });
+    else if (a.out_dtype == COTTUS_F16) each([&](size_t o, float v) { reinterpret_cast<__half*>(a.out)[e + o] = __float2half_rn(v); });
+    else each([&](size_t o, float v) { reinterpret_cast<__nv_bfloat16*>(a.out)[e + o] = __float2bfloat16_rn(v); });
+}
+
 // Position in a ring of n slots and the parity of its current pass.
 struct Ring {
     int slot = 0;
@@ -347,19 +385,21 @@ struct Ring {
     }
 };
 
-// BN: columns of the tile (and of a product buffer).  PAIR: two CTAs share it
-// (the wide tile), else one CTA or a.splits of them (the narrow one).
-template <int BN, bool PAIR>
+// XR: rows of x per CTA.  PAIR: the wide tile, two CTAs of one; else the narrow
+// one, by one CTA or a.splits of them.
+template <int XR, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_constant__ CUtensorMap xmap,
                                                                  const __grid_constant__ CUtensorMap wmap,
                                                                  const __grid_constant__ CUtensorMap omap,
                                                                  const LinArgs a) {
-    static_assert(BN == (PAIR ? 2 : 1) * kWRows, "a CTA brings 128 rows of the weight");
-    constexpr int HALF = BN / 2;
+    static_assert(!PAIR || XR == kBM, "a pair's CTA brings 128 rows of x and of the weight");
+    constexpr int BN = PAIR ? 2 * kWRows : kWRows;   // rows of the weight in a tile
+    constexpr int COLS = PAIR ? BN : XR;             // TMEM columns of a product
+    constexpr int HALF = COLS / 2;                   // and of a sum warp's share
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     // everything in shared memory by 32-bit address
     const uint32_t ring = (smem_addr(smem_raw) + 1023) & ~1023u;
-    const uint32_t stage_bytes = (uint32_t)(a.x_rows + kWRows) * kBK;
+    constexpr uint32_t stage_bytes = (XR + kWRows) * kBK;
     const uint32_t staging = ring + a.stages * stage_bytes;
     const uint32_t scales = staging + a.staging_bytes;
     const uint32_t full = scales + kScaleSlots * kScaleBatch * kScaleWords * 4;
@@ -376,10 +416,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
     uint32_t* s_run = s_tmem + 4;              // splits: where a run of 4 columns is summed up (cluster address)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int splits = PAIR ? 1 : a.splits;
-    // splits have few groups, and with half of the TMEM the next launch's CTA
-    // can allocate its own while this one runs
-    const int bufs = PAIR || splits > 1 ? 2 : 4;
-    const uint32_t tmem_cols = bufs * BN;
+    // (splits have few groups, and with half of the TMEM the next launch's CTA
+    // can allocate its own while this one runs)
+    const int bufs = PAIR || (XR == 128 && splits > 1) ? 2 : 4;
+    const uint32_t tmem_cols = bufs * COLS;
     const int cluster = PAIR ? 2 : splits;
     const int rank = cluster > 1 ? (int)cluster_rank() : 0;
     const int first = blockIdx.x / cluster, step = gridDim.x / cluster;
@@ -388,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
     const int g0 = PAIR ? 0 : (int)((long long)a.groups * rank / splits);
     const int g1 = PAIR ? a.groups : (int)((long long)a.groups * (rank + 1) / splits);
     // first row of x, and first column, of tile t in this CTA
-    auto tile_m = [&](int t) { return PAIR ? (t % a.m_tiles * 2 + rank) * kBM : t % a.m_tiles * kBM; };
+    auto tile_m = [&](int t) { return PAIR ? (t % a.m_tiles * 2 + rank) * kBM : t % a.m_tiles * XR; };
     auto tile_n = [&](int t) { return t / a.m_tiles * BN; };
 
     if (threadIdx.x == 0) {
@@ -412,10 +452,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
     }
     if (warp == kSumWarps + 1) tmem_alloc<PAIR>(words, tmem_cols);
     if (!PAIR && splits > 1 && warp == kSumWarps + 2) {
-        // run r of 32 belongs to split r * splits / 32; its sums lie at
-        // [run][split][row] there, 16 bytes of padding per run
+        // run r of 32 (4 rows of the weight each) belongs to split r * splits
+        // / 32; its sums lie at [split][row of x][run] there
         const int q = (lane * splits) >> 5;
-        s_run[lane] = cluster_addr(staging, q) + (lane - first_run(q, splits)) * (splits * a.x_rows + 1) * 16;
+        s_run[lane] = cluster_addr(staging, q) + (lane - first_run(q, splits)) * 16;
     }
     tc_before();
     __syncthreads();
@@ -455,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
                         const uint32_t at = PAIR ? cluster_addr(bar, 0) : bar;
                         if (!PAIR || rank == 0) bar_expect(bar, (PAIR ? 2 : 1) * stage_bytes);
                         tma_load<PAIR>(st, &xmap, at, g * kBK, m0);
-                        tma_load<PAIR>(st + a.x_rows * kBK, &wmap, at, g * kBK, w0);
+                        tma_load<PAIR>(st + XR * kBK, &wmap, at, g * kBK, w0);
                     }
                     __syncwarp();
                     ++issued;
@@ -479,17 +519,17 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
             }
         } else if (warp == kSumWarps + 1 && !(PAIR && rank)) {
             // ---- MMA issue -----------------------------------------------
-            constexpr uint32_t idesc = f8_idesc<(PAIR ? 2 : 1) * kBM, BN>();
+            constexpr uint32_t idesc = PAIR ? f8_idesc<2 * kBM, BN>() : f8_idesc<kWRows, XR>();
             Ring r, b;
             const uint64_t xdesc = sw128_kmajor_desc(ring);
-            const uint64_t wdesc = sw128_kmajor_desc(ring + a.x_rows * kBK);
+            const uint64_t wdesc = sw128_kmajor_desc(ring + XR * kBK);
             for (int t = first; t < tiles && ok; t += step) {
                 for (int g = g0; g < g1; ++g) {
                     // (descriptors count 16 bytes; the sums' release comes
                     // last and is what the multiplies usually wait for)
                     const uint32_t off = r.slot * (stage_bytes / 16);
-                    const uint64_t ad = xdesc + off, bd = wdesc + off;
-                    const uint32_t d = tmem + (uint32_t)(b.slot * BN);
+                    const uint64_t ad = (PAIR ? xdesc : wdesc) + off, bd = (PAIR ? wdesc : xdesc) + off;
+                    const uint32_t d = tmem + (uint32_t)(b.slot * COLS);
                     ok = bar_wait(full + r.slot * 8, r.phase) && bar_wait(tm_empty + b.slot * 8, b.phase ^ 1);
                     if (!ok) break;
                     tc_after();
@@ -516,9 +556,11 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
             const int part = warp - kSumWarps - 2;
             Ring r;
             for (int t = first; t < tiles && ok; t += step) {
-                const int m = tile_m(t) + part * 64 + lane, nb = tile_n(t) / 128 + lane;
-                const bool live0 = m < a.M, live1 = m + 32 < a.M;
-                const bool live_w = part == 0 && lane < BN / 128 && nb < a.n_blocks;
+                // (the wide tile keeps its two weight scales apart; the narrow
+                // one's single scale goes into the rows')
+                const int r0 = part * 64 + lane, m = tile_m(t) + r0, nb = tile_n(t) / 128 + (PAIR ? lane : 0);
+                const bool live0 = r0 < XR && m < a.M, live1 = r0 + 32 < XR && m + 32 < a.M;
+                const bool live_w = PAIR ? part == 0 && lane < BN / 128 && nb < a.n_blocks : live0 || live1;
                 const float* xs = a.xs + m;
                 const float* ws = a.ws + (size_t)nb * a.groups;
                 for (int gb = g0; gb < g1 && ok; gb += kScaleBatch) {
@@ -535,9 +577,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
 #pragma unroll
                     for (int j = 0; j < kScaleBatch; ++j) {
                         const uint32_t dst = scales + ((r.slot * kScaleBatch + j) * kScaleWords + lane) * 4;
-                        st_shared_f(dst + part * 256, v0[j]);
-                        st_shared_f(dst + part * 256 + 128, v1[j]);
-                        if (part == 0 && lane < BN / 128) st_shared_f(dst + kBM * 4, w[j]);
+                        if (r0 < XR) st_shared_f(dst + part * 256, PAIR ? v0[j] : v0[j] * w[j]);
+                        if (r0 + 32 < XR) st_shared_f(dst + part * 256 + 128, PAIR ? v1[j] : v1[j] * w[j]);
+                        if (PAIR && part == 0 && lane < BN / 128) st_shared_f(dst + kBM * 4, w[j]);
                     }
                     __syncwarp();
                     if (lane == 0) bar_arrive(sc_full + r.slot * 8);
@@ -559,7 +601,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
         if (!PAIR && cluster > 1) cluster_wait();
         Ring b, r;
         for (int t = first; t < tiles && ok; t += step) {
-            const int m0 = tile_m(t) + quad * 32, nh = tile_n(t) + half * HALF;
+            // this warp's first row of x and of the weight
+            const int m0 = tile_m(t) + (PAIR ? quad * 32 : half * HALF), nh = tile_n(t) + (PAIR ? half * HALF : quad * 32);
             const bool rows_live = m0 < a.M;  // (uniform in the warp)
             float2 acc[HALF / 2];
 #pragma unroll
@@ -567,14 +610,14 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
             for (int gb = g0; gb < g1; gb += kScaleBatch) {
                 ok = bar_wait(sc_full + r.slot * 8, r.phase);
                 if (!ok) break;
-                // (the weight's scale is the same word for the whole warp)
+                const uint32_t sc = scales + r.slot * (kScaleBatch * kScaleWords * 4);
                 float sg[kScaleBatch];
-                {
-                    const uint32_t sc = scales + r.slot * (kScaleBatch * kScaleWords * 4);
+                if constexpr (PAIR) {
+                    // (the weight's scale is the same word for the whole warp)
 #pragma unroll
                     for (int j = 0; j < kScaleBatch; ++j)
                         sg[j] = ld_shared_f(sc + (j * kScaleWords + quad * 32 + lane) * 4) *
-                                ld_shared_f(sc + (j * kScaleWords + kBM + (BN > 128 ? half : 0)) * 4);
+                                ld_shared_f(sc + (j * kScaleWords + kBM + half) * 4);
                     __syncwarp();
                     if (lane == 0) mbar_release<false>(sc_empty + r.slot * 8);
                     r.next(kScaleSlots);
@@ -582,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
 #pragma unroll
                 for (int j = 0; j < kScaleBatch; ++j) {
                     if (gb + j >= g1) break;
-                    const uint32_t at = taddr + (uint32_t)(b.slot * BN);
+                    const uint32_t at = taddr + (uint32_t)(b.slot * COLS);
                     const uint32_t freed = tm_free + b.slot * 8;
                     ok = bar_wait(tm_full + b.slot * 8, b.phase);
                     if (!ok) break;
@@ -590,43 +633,62 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
                     tc_after();
                     if (rows_live) {
                         // the next 32 columns are on their way while these are
-                        // added (a load takes about 75 cycles whatever its
-                        // width); the buffer is free once the last ones are here
-                        const float2 s2 = make_float2(sg[j], sg[j]);
+                        // added (a load takes about 75 cycles whatever its width);
+                        // the buffer is free once the last ones are here
+                        constexpr int W = HALF < 32 ? HALF : 32;
                         uint32_t v[2][32];
-                        tmem_ld32(at, v[0]);
+                        if constexpr (W == 8) tmem_get8(at, v[0]);
+                        else if constexpr (W == 16) tmem_get16(at, v[0]);
+                        else tmem_ld32(at, v[0]);
 #pragma unroll
-                        for (int i = 0; i < HALF / 32; ++i) {
-                            tmem_wait_ld(v[i & 1]);
-                            if (i + 1 < HALF / 32) {
+                        for (int i = 0; i < HALF / W; ++i) {
+                            if constexpr (W == 32) tmem_wait_ld(v[i & 1]);
+                            if (i + 1 < HALF / W) {
                                 tmem_ld32(at + (uint32_t)(i + 1) * 32, v[(i + 1) & 1]);
                             } else {
                                 tc_before();
                                 if (lane == 0) mbar_release<PAIR>(freed);
                             }
 #pragma unroll
-                            for (int c = 0; c < 16; ++c)
-                                acc[i * 16 + c] = ffma2(
-                                    make_float2(__uint_as_float(v[i & 1][2 * c]), __uint_as_float(v[i & 1][2 * c + 1])),
-                                    s2, acc[i * 16 + c]);
+                            for (int c = 0; c < W; c += 4) {
+                                float2 sa, sb;
+                                if constexpr (PAIR) {
+                                    sa = sb = make_float2(sg[j], sg[j]);
+                                } else {
+                                    const float4 s4 = ld_shared_f4(sc + (j * kScaleWords + half * HALF + i * W + c) * 4);
+                                    sa = make_float2(s4.x, s4.y);
+                                    sb = make_float2(s4.z, s4.w);
+                                }
+                                const uint32_t(&u)[32] = v[i & 1];
+                                float2 &ta = acc[(i * W + c) / 2], &tb = acc[(i * W + c) / 2 + 1];
+                                ta = ffma2(make_float2(__uint_as_float(u[c]), __uint_as_float(u[c + 1])), sa, ta);
+                                tb = ffma2(make_float2(__uint_as_float(u[c + 2]), __uint_as_float(u[c + 3])), sb, tb);
+                            }
                         }
                     } else if (lane == 0) {
                         mbar_release<PAIR>(freed);
                     }
                 }
+                if constexpr (!PAIR) {
+                    __syncwarp();
+                    if (lane == 0) mbar_release<false>(sc_empty + r.slot * 8);
+                    r.next(kScaleSlots);
+                }
                 if (!ok) break;
             }
             if (!ok) break;
             if (!PAIR && splits > 1) {
-                // (the only tile of this cluster) every run of 4 columns goes to
-                // the CTA that sums it up
-                if (m0 + lane < a.M) {
-                    const uint32_t mine = (uint32_t)(rank * a.x_rows + quad * 32 + lane) * 16;
+                // (the only tile of this cluster) every sum goes to the CTA that
+                // adds its weight row up
+                if constexpr (!PAIR) {
+                    const int runs = (32 + splits - 1) / splits, row = quad * 32 + lane;
+                    const uint32_t to = s_run[row >> 2] + (uint32_t)((rank * XR + half * HALF) * runs * 16 + (row & 3) * 4);
 #pragma unroll
-                    for (int c = 0; c < HALF; c += 4)
-                        st_cluster_f4(s_run[(half * HALF + c) / 4] + mine,
-                                      make_float4(acc[c / 2].x, acc[c / 2].y, acc[c / 2 + 1].x, acc[c / 2 + 1].y));
+                    for (int c = 0; c < HALF; ++c)
+                        if (m0 + c < a.M) st_cluster_f(to + c * runs * 16, c & 1 ? acc[c / 2].y : acc[c / 2].x);
                 }
+            } else if constexpr (!PAIR) {
+                if (rows_live) store_column<HALF>(a, m0, nh + lane, acc);
             } else if (a.tma_out) {
                 // 128 bytes of each of the warp's rows at a time, swizzled as
                 // the tensor map has it, stored by TMA (which drops what lies
@@ -705,16 +767,17 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
         cluster_wait();  // every CTA's partial sums are where they are added
         if (!s_failed[1]) {
             const int m0 = tile_m(first), n0 = tile_n(first);
-            const int rows = a.M - m0 < kBM ? a.M - m0 : kBM;
+            const int rows = a.M - m0 < XR ? a.M - m0 : XR;
             const int run0 = first_run(rank, splits), runs = first_run(rank + 1, splits) - run0;
             const int sh = runs > 16 ? 5 : (runs > 8 ? 4 : (runs > 4 ? 3 : 2));  // lanes per row
             const int run = threadIdx.x & ((1 << sh) - 1), n = n0 + (run0 + run) * 4;
             if (run < runs && n < a.N) {
-                const uint32_t p = staging + run * (splits * a.x_rows + 1) * 16;
+                const int pitch = (32 + splits - 1) / splits * 16;
                 for (int row = threadIdx.x >> sh; row < rows; row += kThreads >> sh) {
-                    float4 v = ld_shared_f4(p + row * 16);
+                    const uint32_t p = staging + row * pitch + run * 16;
+                    float4 v = ld_shared_f4(p);
                     for (int q = 1; q < splits; ++q) {
-                        const float4 w = ld_shared_f4(p + (q * a.x_rows + row) * 16);
+                        const float4 w = ld_shared_f4(p + q * XR * pitch);
                         v.x += w.x;
                         v.y += w.y;
                         v.z += w.z;
@@ -744,9 +807,9 @@ struct DeviceLimits {
     int pairs = 0;                      // and wide-tile pairs (not every SM has a partner)
     cudaError_t err = cudaSuccess;
 };
-template <int BN, bool PAIR>
+template <int XR, bool PAIR>
 cudaError_t set_up_kernel() {
-    auto kern = fp8_linear_kernel<BN, PAIR>;
+    auto kern = fp8_linear_kernel<XR, PAIR>;
     cudaFuncAttributes fa = {};
     cudaError_t e = cudaFuncGetAttributes(&fa, kern);
     if (e != cudaSuccess) return e;
@@ -757,8 +820,9 @@ cudaError_t set_up_kernel() {
 DeviceLimits find_limits(int dev) {
     DeviceLimits l;
     l.sms = device_sm_count(dev);
-    l.err = set_up_kernel<128, false>();
-    if (l.err == cudaSuccess) l.err = set_up_kernel<256, true>();
+    for (auto set_up : {set_up_kernel<16, false>, set_up_kernel<32, false>, set_up_kernel<64, false>,
+                        set_up_kernel<128, false>, set_up_kernel<128, true>})
+        if (l.err == cudaSuccess) l.err = set_up();
     auto resident = [&](auto kern, int size, int* n) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(size);
@@ -774,7 +838,7 @@ DeviceLimits find_limits(int dev) {
         if (l.err == cudaSuccess) l.err = cudaOccupancyMaxActiveClusters(n, kern, &cfg);
     };
     for (int s = 1; s <= kMaxSplits; ++s) resident(fp8_linear_kernel<128, false>, s, &l.clusters[s]);
-    resident(fp8_linear_kernel<256, true>, 2, &l.pairs);
+    resident(fp8_linear_kernel<128, true>, 2, &l.pairs);
     return l;
 }
 constexpr int kMaxDevices = 64;
@@ -790,13 +854,12 @@ cudaError_t limits(DeviceLimits& l) {
     return l.err;
 }
 
-template <int BN, bool PAIR>
+template <int XR, bool PAIR>
 cudaError_t launch_linear(const cottus_fp8_linear_params* p, LinArgs a, int grid, cudaStream_t st) {
     cudaError_t err = cudaSuccess;
-    a.x_rows = p->rows < kBM ? (p->rows + 7) / 8 * 8 : kBM;
-    a.staging_bytes = kSumWarps * kWarpStaging;
-    if (a.splits > 1) a.staging_bytes = (32 + a.splits - 1) / a.splits * (a.splits * a.x_rows + 1) * 16;
-    const size_t stage = (size_t)(a.x_rows + kWRows) * kBK;
+    a.staging_bytes = PAIR ? kSumWarps * kWarpStaging : 0;
+    if (a.splits > 1) a.staging_bytes = a.splits * XR * ((32 + a.splits - 1) / a.splits) * 16;
+    const size_t stage = (size_t)(XR + kWRows) * kBK;
     const size_t rest = 1024 + (size_t)a.staging_bytes + kTailBytes;
     a.stages = (int)((kSmemMax - rest) / stage);
     if (a.stages > kMaxStages) a.stages = kMaxStages;
@@ -804,14 +867,14 @@ cudaError_t launch_linear(const cottus_fp8_linear_params* p, LinArgs a, int grid
     // shared memory can become resident beside the one before it
     const int most = (a.groups + a.splits - 1) / a.splits;
     if (a.splits > 1 && a.stages > most) a.stages = most;
-    const CUtensorMap xmap = make_tensor_map_2d_u8(p->x, p->in_features, p->rows, p->in_features, kBK, a.x_rows, true, &err);
+    const CUtensorMap xmap = make_tensor_map_2d_u8(p->x, p->in_features, p->rows, p->in_features, kBK, XR, true, &err);
     if (err != cudaSuccess) return err;
     const CUtensorMap wmap =
         make_tensor_map_2d_u8(p->weight, p->in_features, p->out_features, p->in_features, kBK, kWRows, true, &err);
     if (err != cudaSuccess) return err;
     CUtensorMap omap = wmap;  // (not read without tma_out)
     const int es = dtype_bytes(p->out_dtype);
-    a.tma_out = a.splits == 1 && !p->residual && aligned(p->out, 16) && (size_t)p->out_features * es % 16 == 0;
+    a.tma_out = PAIR && !p->residual && aligned(p->out, 16) && (size_t)p->out_features * es % 16 == 0;
     if (a.tma_out) {
         omap = make_tensor_map_2d_u8(p->out, (uint64_t)p->out_features * es, p->rows, (uint64_t)p->out_features * es, 128, 32,
                                      true, &err);
@@ -831,7 +894,7 @@ cudaError_t launch_linear(const cottus_fp8_linear_params* p, LinArgs a, int grid
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = PAIR || a.splits > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, fp8_linear_kernel<BN, PAIR>, xmap, wmap, omap, a);
+    return cudaLaunchKernelEx(&cfg, fp8_linear_kernel<XR, PAIR>, xmap, wmap, omap, a);
 }
 
 }  // namespace
@@ -886,7 +949,7 @@ extern "C" int cottus_fp8_linear(const cottus_fp8_linear_params* p, cottus_strea
         a.m_tiles = (M + 255) / 256;
         a.n_tiles = (N + 255) / 256;
         a.splits = 1;
-        e = launch_linear<256, true>(p, a, 2 * (int)(wide < dev.pairs ? wide : dev.pairs), st);
+        e = launch_linear<128, true>(p, a, 2 * (int)(wide < dev.pairs ? wide : dev.pairs), st);
     } else {
         a.m_tiles = (M + 127) / 128;
         a.n_tiles = (N + 127) / 128;
@@ -894,8 +957,11 @@ extern "C" int cottus_fp8_linear(const cottus_fp8_linear_params* p, cottus_strea
         a.splits = 1;
         for (int s = 2; s <= kMaxSplits && s <= groups; ++s)
             if (narrow <= dev.clusters[s]) a.splits = s;
-        e = launch_linear<128, false>(p, a, a.splits > 1 ? (int)narrow * a.splits : (int)(narrow < dev.sms ? narrow : dev.sms),
-                                      st);
+        const int grid = a.splits > 1 ? (int)narrow * a.splits : (int)(narrow < dev.sms ? narrow : dev.sms);
+        e = M <= 16   ? launch_linear<16, false>(p, a, grid, st)
+            : M <= 32 ? launch_linear<32, false>(p, a, grid, st)
+            : M <= 64 ? launch_linear<64, false>(p, a, grid, st)
+                      : launch_linear<128, false>(p, a, grid, st);
     }
     return e == cudaSuccess ? COTTUS_OK : fail(COTTUS_ERR_CUDA, std::string("CUDA error: ") + cudaGetErrorString(e));
 }
