@@ -438,6 +438,50 @@ def sample_tokens(logits, uniforms, *, temperature=None, top_k=None, top_p=None,
     return (out, logprobs) if return_logprobs else out
 
 
+def attention_block_fp8(batch, residual, norm_weight, w_qkv, qkv_scales, w_o, o_scales, kv_pool, cos_sin, *, num_heads,
+                        num_kv_heads, head_dim, eps=1e-5, num_layers=1, layer=0, status=None, stream=None):
+    """attention_block on 8-bit weights, the norm in front included: for the step tokens of a DecodeBatch, from the
+    residual stream back into it (generic_transformer.cpp:154-327 per token), as launches of this library: rms_norm to
+    e4m3, the q, k and v projections (fp8_linear over row ranges of w_qkv), RoPE + append + paged decode
+    (rope_append_decode), quantize_fp8 and the output projection added to the stream in place.
+
+    residual [n][hidden] fp32 (updated), w_qkv [(H + 2 Hkv) D][hidden] and w_o [hidden][H D] e4m3 with the scales of
+    quantize_fp8(block_rows=128); H D and Hkv D multiples of 128 (a range starts at a scale block).  Returns the
+    attention output [n][H D] fp16."""
+    n, qd, kd = len(batch), num_heads * head_dim, num_kv_heads * head_dim
+    if residual.shape[0] != n:
+        raise ValueError(f"residual needs one row per active sequence ({n})")
+    if qd % 128 or kd % 128:
+        raise ValueError("num_heads * head_dim and num_kv_heads * head_dim must be multiples of 128")
+    if w_qkv.shape[0] != qd + 2 * kd:
+        raise ValueError(f"w_qkv must have {qd + 2 * kd} rows")
+    h, hs = rms_norm(residual, norm_weight, eps=eps, out_dtype=_FP8, stream=stream)
+    qkv = []
+    for r0, rows, heads in ((0, qd, num_heads), (qd, kd, num_kv_heads), (qd + kd, kd, num_kv_heads)):
+        part = fp8_linear(h, hs, w_qkv[r0:r0 + rows], qkv_scales[r0 // 128:(r0 + rows) // 128], status=status,
+                          stream=stream)
+        qkv.append(part.view(n, heads, head_dim))
+    att = rope_append_decode(*qkv, batch.positions[:n], cos_sin, kv_pool, batch.block_table[:n],
+                             num_kv_heads=num_kv_heads, head_dim=head_dim, block_size=batch.block_size,
+                             num_layers=num_layers, layer=layer, status=status, stream=stream).view(n, qd)
+    a, a_scales = quantize_fp8(att, stream=stream)
+    fp8_linear(a, a_scales, w_o, o_scales, residual=residual, out=residual, status=status, stream=stream)
+    return att
+
+
+def next_tokens(residual, norm_weight, w_head, head_scales, uniforms, *, eps=1e-5, temperature=None, top_k=None,
+                top_p=None, min_p=None, logits=None, tokens=None, status=None, stream=None):
+    """The end of a decode step (generic_transformer.cpp:369-370 and the argmax of engine.cpp:85-87), from the residual
+    stream [n][hidden] fp32 to one token per row: the final rms_norm to e4m3, the vocabulary projection (fp8_linear,
+    w_head [vocab][hidden] e4m3 with the scales of quantize_fp8(block_rows=128)) and sample_tokens.  Returns
+    (tokens int32 [n], logits fp32 [n][vocab])."""
+    h, hs = rms_norm(residual, norm_weight, eps=eps, out_dtype=_FP8, stream=stream)
+    logits = fp8_linear(h, hs, w_head, head_scales, out=logits, out_dtype=torch.float32, status=status, stream=stream)
+    tokens = sample_tokens(logits, uniforms, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, out=tokens,
+                           status=status, stream=stream)
+    return tokens, logits
+
+
 def paged_gather(kv_pool, block_table, context_lens, *, max_context, num_kv_heads, head_dim, block_size,
                  num_layers=1, layer=0, num_physical_blocks=None, status=None, k_out=None, v_out=None, stream=None):
     """Dense copy of the K and V rows named by the block table (bit-exact)."""
