@@ -311,6 +311,11 @@ def _raw_stream(stream, device: int):
 _ONLY_F32, _ONLY_I32, _ONLY_FP8 = (torch.float32,), (torch.int32,), (_FP8,)
 
 
+def _new(like: torch.Tensor, rows: int, cols: int, dtype) -> torch.Tensor:
+    """A contiguous [rows][cols] tensor (empty_strided parses its arguments in half the time of new_empty, 1.8 us)."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=like.device)
+
+
 def rms_norm(x, weight, *, eps=1e-5, residual=None, residual_out=None, out=None, out_dtype=None, scales=None,
              stream=None):
     """RMS norm with the residual's addition (cottus_rms_norm):
@@ -340,7 +345,7 @@ def rms_norm(x, weight, *, eps=1e-5, residual=None, residual_out=None, out=None,
     p.out = _operand(out, "out", x.shape, _ONLY_FP8 if fp8 else _DT_WIDE, dev)
     if fp8:
         if scales is None:
-            scales = x.new_empty(((hidden + 127) // 128, rows), dtype=torch.float32)
+            scales = _new(x, (hidden + 127) // 128, rows, torch.float32)
         p.scales = _operand(scales, "scales", ((hidden + 127) // 128, rows), _ONLY_F32, dev)
     elif scales is not None:
         raise ValueError("scales go with a torch.float8_e4m3fn output")
@@ -365,7 +370,7 @@ def quantize_fp8(x, *, block_rows=1, out=None, scales=None, stream=None):
     groups = (cols + 127) // 128
     shape = ((rows + 127) // 128, groups) if block_rows == 128 else (groups, rows)
     if scales is None:
-        scales = x.new_empty(shape, dtype=torch.float32)
+        scales = _new(x, *shape, torch.float32)
     p.out = _operand(out, "out", x.shape, _ONLY_FP8, dev)
     p.scales = _operand(scales, "scales", shape, _ONLY_F32, dev)
     p.rows, p.cols, p.x_dtype, p.block_rows = rows, cols, _DT_WIDE[x.dtype], block_rows
@@ -392,7 +397,7 @@ def fp8_linear(x, x_scales, weight, weight_scales, *, residual=None, out=None, o
     if residual is not None:
         p.residual = _operand(residual, "residual", (rows, fout), _ONLY_F32, dev)
     if out is None:
-        out = x.new_empty((rows, fout), dtype=out_dtype)
+        out = _new(x, rows, fout, out_dtype)
     p.out = _operand(out, "out", (rows, fout), _DT_WIDE, dev)
     p.rows, p.out_features, p.in_features, p.out_dtype = rows, fout, fin, _DT_WIDE[out.dtype]
     if status is not None:

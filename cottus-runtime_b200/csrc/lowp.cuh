@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "cottus_b200.h"
@@ -68,6 +69,18 @@ __device__ __forceinline__ void load8_stream(const __nv_bfloat16* p, float (&v)[
     }
 }
 
+// Maximum that keeps a NaN of either side.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float amax8(const float (&v)[8]) {
+    float m = fabsf(v[0]);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
+    return m;
+}
 // Eight elements in their own type.
 template <typename XT>
 struct Vec8 {
@@ -89,6 +102,29 @@ struct Vec8 {
         if constexpr (sizeof(XT) == 4) w[j] = __float_as_uint(to_f32(x));
         else h[j] = *reinterpret_cast<uint16_t*>(&x);
     }
+    // Largest magnitude (NaN kept); two 16-bit values per operation.
+    __device__ __forceinline__ float amax() const {
+        if constexpr (sizeof(XT) == 4) {
+            float v[8];
+            get(v);
+            return amax8(v);
+        } else {
+            const uint32_t m = max2_abs(max2_abs(w[0], w[1]), max2_abs(w[2], w[3]));
+            return max_nan(to_f32(half_of(m)), to_f32(half_of(m >> 16)));
+        }
+    }
+    __device__ __forceinline__ static XT half_of(uint32_t x) {
+        const uint16_t b = (uint16_t)x;
+        return *reinterpret_cast<const XT*>(&b);
+    }
+    __device__ __forceinline__ static uint32_t max2_abs(uint32_t a, uint32_t b) {
+        a &= 0x7FFF7FFFu;
+        b &= 0x7FFF7FFFu;
+        uint32_t r;
+        if constexpr (std::is_same<XT, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
     __device__ __forceinline__ void get(float (&v)[8]) const {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -98,18 +134,6 @@ struct Vec8 {
     }
 };
 
-// Maximum that keeps a NaN of either side.
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float amax8(const float (&v)[8]) {
-    float m = fabsf(v[0]);
-#pragma unroll
-    for (int j = 1; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
-    return m;
-}
 // Maximum over each half of the warp (all 32 lanes take part).
 __device__ __forceinline__ float amax16(float m) {
 #pragma unroll
@@ -129,18 +153,23 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 // RN(v / s) (Markstein, IBM J. Res. Dev. 34, 1990) while nothing underflows:
 // v below 2^-10 s is 0 in e4m3 whatever its last bit, and for larger v the
 // remainder stays a normal number where s >= 2^-90.  Smaller, infinite and NaN
-// scales divide.  Three packed operations for two quotients instead of two
-// divisions: the 28672 x 8200 bf16 weight took 272 us with divisions.
+// scales divide.  (With divisions the 28672 x 8200 bf16 weight took 272 us.)
 struct Divisor {
     float s, r;
     bool plain;
     __device__ __forceinline__ explicit Divisor(float scale) : s(scale), r(0.f), plain(scale >= 0x1p-90f && scale < INFINITY) {
         if (plain) r = __frcp_rn(scale);
     }
+    __device__ __forceinline__ float quotient(float v) const {
+        if (!plain) return __fdiv_rn(v, s);
+        const float q0 = v * r;
+        return fmaf(fmaf(-q0, s, v), r, q0);
+    }
 };
 __device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], const Divisor& d) {
     float q[8];
     if (d.plain) {
+        // (two at a time: the 28672 x 8200 weight takes 133 us, one by one 146)
         const float2 r2 = make_float2(d.r, d.r), ns2 = make_float2(-d.s, -d.s);
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
@@ -159,7 +188,7 @@ __device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], const Divisor& d) {
     o.y = e4m3x2(q[4], q[5]) | (e4m3x2(q[6], q[7]) << 16);
     return o;
 }
-__device__ __forceinline__ uint8_t e4m3(float v, float s) { return (uint8_t)(e4m3x2(__fdiv_rn(v, s), 0.f) & 0xFFu); }
+__device__ __forceinline__ uint8_t e4m3(float v, const Divisor& d) { return (uint8_t)(e4m3x2(d.quotient(v), 0.f) & 0xFFu); }
 
 // ---------------------------------------------------------------------------
 // host
