@@ -327,9 +327,11 @@ cudaError_t launch_quant(const QuantArgs& a, bool blocks, cudaStream_t st) {
     // four groups per thread once the small tiles fill the GPU's 8 CTAs per SM:
     // 16384 x 8192 fp16 84 us against 117, 64 x 4096 (128 small tiles) 2.2 against
     // 1.5.  Element by element they do not help (8192 x 8191 bf16 117 against 79).
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (VEC && (a.rows + 15) / 16 * groups >= 8LL * device_sm_count(dev)) return rows(quant_rows_kernel<XT, VEC, 2, 2>, 2, 2);
+    if constexpr (VEC) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if ((a.rows + 15) / 16 * groups >= 8LL * device_sm_count(dev)) return rows(quant_rows_kernel<XT, true, 2, 2>, 2, 2);
+    }
     return rows(quant_rows_kernel<XT, VEC, 1, 1>, 1, 1);
 }
 

@@ -136,7 +136,8 @@ def test_rms_norm_special_rows(hidden):
     assert torch.isnan(cb.rms_norm(x.to(DEV), w.to(DEV), eps=0.0).cpu()[0]).all()
 
 
-QUANT_SHAPES = [(1, 128), (1, 1), (3, 5), (128, 128), (129, 257), (130, 264), (64, 4096), (5, 8200), (300, 72), (2, 8)]
+QUANT_SHAPES = [(1, 128), (1, 1), (3, 5), (128, 128), (129, 257), (130, 264), (64, 4096), (5, 8200), (300, 72), (2, 8),
+                (700, 4104), (1001, 2600)]
 
 
 @pytest.mark.parametrize("rows, cols", QUANT_SHAPES)
