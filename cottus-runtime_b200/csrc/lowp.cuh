@@ -140,7 +140,14 @@ __device__ __forceinline__ float amax16(float m) {
     for (int o = 8; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     return m;
 }
-__device__ __forceinline__ float group_scale(float amax) { return max_nan(__fdiv_rn(amax, kE4m3Max), kMinScale); }
+// max(amax / 448, 2^-126), the quotient correctly rounded as below (what a
+// subnormal remainder would spoil is under the smallest scale anyway).
+__device__ __forceinline__ float group_scale(float amax) {
+    constexpr float r = 1.f / kE4m3Max;
+    const float q0 = amax * r;
+    const float q = fmaf(fmaf(-q0, kE4m3Max, amax), r, q0);
+    return amax < INFINITY ? fmaxf(q, kMinScale) : amax;
+}
 
 // value / scale in e4m3, to nearest even, magnitudes above 448 to 448, NaN kept.
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
@@ -186,6 +193,16 @@ __device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], const Divisor& d) {
     uint2 o;
     o.x = e4m3x2(q[0], q[1]) | (e4m3x2(q[2], q[3]) << 16);
     o.y = e4m3x2(q[4], q[5]) | (e4m3x2(q[6], q[7]) << 16);
+    return o;
+}
+// Eight values times the reciprocal of their group's scale: for values that
+// are rounded themselves, as a norm's are, where the quotient's last fp32 bit
+// is below their own error.
+__device__ __forceinline__ uint2 e4m3x8_times(const float (&v)[8], const Divisor& d) {
+    if (!d.plain) return e4m3x8(v, d);
+    uint2 o;
+    o.x = e4m3x2(v[0] * d.r, v[1] * d.r) | (e4m3x2(v[2] * d.r, v[3] * d.r) << 16);
+    o.y = e4m3x2(v[4] * d.r, v[5] * d.r) | (e4m3x2(v[6] * d.r, v[7] * d.r) << 16);
     return o;
 }
 __device__ __forceinline__ uint8_t e4m3(float v, const Divisor& d) { return (uint8_t)(e4m3x2(d.quotient(v), 0.f) & 0xFFu); }

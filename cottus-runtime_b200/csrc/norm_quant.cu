@@ -122,7 +122,7 @@ __global__ void rms_norm_vec_kernel(const NormArgs a) {
         }
         const float s = group_scale(amax16(amax8(h[i])));
         if (live) {
-            *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.out) + e) = e4m3x8(h[i], Divisor(s));
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.out) + e) = e4m3x8_times(h[i], Divisor(s));
             if ((v & 15) == 0) a.scales[(size_t)(v >> 4) * a.rows + row] = s;
         }
     }
