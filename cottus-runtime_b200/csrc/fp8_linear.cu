@@ -80,6 +80,7 @@ constexpr int kScaleBatch = 4;
 constexpr int kPrefetch = 4;   // groups whose weights are prefetched into L2
 constexpr int kScaleWords = kBM + 4;  // a group's scales: 128 rows, then one per 128 columns of the tile
 constexpr size_t kSmemMax = 232448;   // dynamic shared memory per CTA, 227 KB
+constexpr size_t kSplitSmem = 115712;  // half of an SM's, 113 KB: at least this for splits
 constexpr int kWarpStaging = 32 * 128;  // per sum warp: 128 bytes of each of its rows (or 16 padded columns)
 // scales, barriers and words behind the ring and the staging area
 constexpr size_t kTailBytes =
@@ -884,6 +885,15 @@ cudaError_t launch_linear(const cottus_fp8_linear_params* p, LinArgs a, int grid
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = rest + (size_t)a.stages * stage;
+    // A cluster's CTAs wait for one another with their tensor memory allocated,
+    // and an allocation waits for as long as it takes: CTAs of two such kernels
+    // that met on the same SMs in opposite order could hold what the other one
+    // needs.  The wide tile's registers (64512 of 65536) keep everything else
+    // off its SMs; splits take half of an SM's shared memory, so that a kernel
+    // that uses the rest of it for its own multiplies does not join them (two
+    // of these do: with 256 columns each at most their tensor memory fits).
+    // Decode projections take the same time with it.
+    if (a.splits > 1 && cfg.dynamicSmemBytes < kSplitSmem) cfg.dynamicSmemBytes = kSplitSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -915,6 +925,7 @@ extern "C" int cottus_fp8_linear(const cottus_fp8_linear_params* p, cottus_strea
     if (!aligned(p->out, es) || !aligned(p->residual, 4) || !aligned(p->x_scales, 4) || !aligned(p->w_scales, 4))
         return fail(COTTUS_ERR_INVALID_ARGUMENT, "a pointer is not aligned to its element");
     const int M = p->rows, N = p->out_features, K = p->in_features;
+    if (M > kMaxWidth || N > kMaxWidth || K > kMaxWidth) return fail(COTTUS_ERR_UNSUPPORTED, "product too large");
     const int groups = (K + 127) / 128;
     const size_t mn = (size_t)M * N;
     const Span so{p->out, mn * es}, sr{p->residual, p->residual ? mn * 4 : 0}, sx{p->x, (size_t)M * K},

@@ -210,6 +210,7 @@ __device__ __forceinline__ uint8_t e4m3(float v, const Divisor& d) { return (uin
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
+constexpr int kMaxWidth = 1 << 30;  // of a matrix: the kernels round 32-bit columns up to whole tiles
 inline bool lowp_input_dtype(int32_t t) { return t == COTTUS_F32 || t == COTTUS_F16 || t == COTTUS_BF16; }
 inline int dtype_bytes(int32_t t) { return t == COTTUS_F32 ? 4 : (t == COTTUS_E4M3 ? 1 : 2); }
 inline bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }

@@ -358,6 +358,7 @@ int cottus_rms_norm(const cottus_rms_norm_params* p, cottus_stream_t stream) {
     if ((p->out_dtype == COTTUS_E4M3) != (p->scales != nullptr))
         return fail(COTTUS_ERR_INVALID_ARGUMENT, "scales go with an e4m3 output, and only with one");
     if (p->rows >= (int64_t(1) << 31)) return fail(COTTUS_ERR_UNSUPPORTED, "too many rows for one launch");
+    if (p->hidden > kMaxWidth) return fail(COTTUS_ERR_UNSUPPORTED, "hidden is too large");
     const size_t n = (size_t)p->rows * p->hidden;
     const int xs = dtype_bytes(p->x_dtype), os = dtype_bytes(p->out_dtype);
     const size_t sb = p->scales ? (size_t)p->rows * ((p->hidden + 127) / 128) * 4 : 0;
@@ -399,8 +400,9 @@ int cottus_quantize_fp8(const cottus_quantize_params* p, cottus_stream_t stream)
     if (p->block_rows != 1 && p->block_rows != 128) return fail(COTTUS_ERR_INVALID_ARGUMENT, "block_rows must be 1 or 128");
     if (p->rows == 0) return COTTUS_OK;
     if (!p->x || !p->out || !p->scales) return fail(COTTUS_ERR_INVALID_ARGUMENT, "NULL pointer argument");
+    if (p->cols > kMaxWidth) return fail(COTTUS_ERR_UNSUPPORTED, "cols is too large");
     const bool blocks = p->block_rows == 128;
-    const int64_t groups = (p->cols + 127) / 128, row_blocks = (p->rows + 127) / 128;
+    const int64_t groups = (p->cols + 127) / 128, row_blocks = p->rows / 128 + (p->rows % 128 != 0);
     if (blocks ? row_blocks > 65535 : (p->rows >> 4) >= (int64_t(1) << 31) / groups - 1)
         return fail(COTTUS_ERR_UNSUPPORTED, "too many rows for one launch");
     const size_t n = (size_t)p->rows * p->cols;

@@ -107,9 +107,6 @@ __device__ __forceinline__ uint32_t mapa(const void* local, uint32_t rank) {
 __device__ __forceinline__ void st_cluster(uint32_t a, u64 v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
-__device__ __forceinline__ void st_cluster(uint32_t a, uint32_t v) {
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
-}
 __device__ __forceinline__ uint32_t ld_cluster(uint32_t a) {
     uint32_t v;
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");

@@ -296,7 +296,9 @@ int cottus_o_proj_residual(const cottus_o_proj_params *p, cottus_stream_t stream
  * (448 = the largest e4m3 value); stored value = value / scale rounded to
  * nearest even, at most 448 in magnitude.  A NaN anywhere in a group makes
  * the group's scale and values NaN; an infinity makes the scale infinite,
- * the infinities NaN and the finite values 0.
+ * the infinities NaN and the finite values 0.  (cottus_rms_norm multiplies by
+ * the scale's reciprocal: its values are rounded numbers themselves.)
+ * A row or column count above 2^30 is refused.
  * Each call is one kernel, stream-ordered, without workspace; every call may
  * be captured in a CUDA graph and replayed.  Buffers must not overlap unless
  * a field says so.  rows or batch 0 is a successful no-op.
@@ -338,7 +340,8 @@ int cottus_quantize_fp8(const cottus_quantize_params *p, cottus_stream_t stream)
 /* Block-scaled e4m3 matrix product on the tensor cores:
  *   out[m][n] = sum_b x_scales[b][m] * w_scales[n/128][b] *
  *               sum_{k in group b} x[m][k] * weight[n][k]   (+ residual[m][n])
- * with fp32 accumulation; x in the activation layout, weight ([out][in], as
+ * with fp32 accumulation (the two scales' product is formed first: it should
+ * be a normal fp32 number); x in the activation layout, weight ([out][in], as
  * in cottus_o_proj_residual) in the weight layout.  in_features a multiple of
  * 16, any out_features and any number of rows (a decode batch or a prefill
  * chunk).  Replaces gemmCUDA (compute_primitives_cuda.cu:30-55) and, with
@@ -372,8 +375,9 @@ int cottus_fp8_linear(const cottus_fp8_linear_params *p, cottus_stream_t stream)
  *      the front candidate always stays;
  *   5. the token is the first one, in index order, at which the running sum
  *      of the kept weights exceeds uniform * their sum.
- * The weights are computed in fp64 and summed as 64-bit fixed-point numbers,
- * so a result does not depend on the order of the additions.
+ * A weight is off by at most 2^-31 of itself or 2^-43 of the largest one, and
+ * the sums are of 64-bit fixed-point numbers, so a result does not depend on
+ * the order of the additions.
  * temperature <= 0 or NaN takes the front candidate.  top_k <= 0, top_p >= 1
  * or NaN, min_p <= 0 or NaN switch that filter off; top_p <= 0 or min_p > 1
  * keep the front candidate only.  uniform is clamped into [0, 1).  A row
