@@ -189,8 +189,9 @@ def rope_append(query, key, value, positions, cos_sin, kv_pool, block_table, *, 
 
 def rope_append_decode(query, key, value, positions, cos_sin, kv_pool, block_table, *, num_kv_heads, head_dim,
                        block_size, num_layers=1, layer=0, out=None, out_dtype=None, query_out=None, scale=0.0,
-                       status=None, stream=None):
-    """RoPE + KV append + paged attention over positions+1 tokens (one kernel)."""
+                       status=None, stream=None, workspace_of=None):
+    """RoPE + KV append + paged attention over positions+1 tokens (one kernel).  workspace_of: the DecodeBatch whose
+    workspace serves the call; by default all calls on a device share one, and must not overlap on several streams."""
     for t, n in ((query, "query"), (key, "key"), (value, "value"), (kv_pool, "kv_pool")):
         _require(t, n)
     if out is None:
@@ -200,7 +201,7 @@ def rope_append_decode(query, key, value, positions, cos_sin, kv_pool, block_tab
                          query_out=query_out, out=out, scale=scale, status=status)
     need = lib().cottus_rope_append_decode_workspace_size(C.byref(p))
     if need:
-        ws = workspace(need, query.device)
+        ws = workspace(need, query.device) if workspace_of is None else workspace_of.workspace(need)
         p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
     check(lib().cottus_rope_append_decode(C.byref(p), _stream(stream)))
     return out
@@ -311,9 +312,21 @@ def _raw_stream(stream, device: int):
 _ONLY_F32, _ONLY_I32, _ONLY_FP8 = (torch.float32,), (torch.int32,), (_FP8,)
 
 
-def _new(like: torch.Tensor, rows: int, cols: int, dtype) -> torch.Tensor:
-    """A contiguous [rows][cols] tensor (empty_strided parses its arguments in half the time of new_empty, 1.8 us)."""
-    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=like.device)
+def _new(like: torch.Tensor, shape, dtype, stream) -> torch.Tensor:
+    """A contiguous tensor of one or two dimensions (empty_strided parses its arguments in half the time of new_empty,
+    1.8 us), of the memory pool of the stream that writes it: of another's it might hold what that one still reads."""
+    strides = (shape[1], 1) if len(shape) == 2 else (1,)
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return torch.empty_strided(shape, strides, dtype=dtype, device=like.device)
+    return torch.empty_strided(shape, strides, dtype=dtype, device=like.device)
+
+
+def _i32(n: int, name: str) -> int:
+    """n as the C ABI's 32-bit sizes hold it (ctypes would drop the upper bits)."""
+    if not 0 <= n < 1 << 31:
+        raise ValueError(f"{name} is {n}, a 32-bit size")
+    return n
 
 
 def rms_norm(x, weight, *, eps=1e-5, residual=None, residual_out=None, out=None, out_dtype=None, scales=None,
@@ -338,18 +351,19 @@ def rms_norm(x, weight, *, eps=1e-5, residual=None, residual_out=None, out=None,
     elif residual_out is not None:
         raise ValueError("residual_out goes with residual")
     if out is None:
-        out = torch.empty_like(x, dtype=out_dtype)
+        out = _new(x, (rows, hidden), out_dtype or x.dtype, stream)
     elif out_dtype is not None and out.dtype != out_dtype:
         raise TypeError(f"out is {out.dtype}, out_dtype is {out_dtype}")
     fp8 = out.dtype == _FP8
     p.out = _operand(out, "out", x.shape, _ONLY_FP8 if fp8 else _DT_WIDE, dev)
     if fp8:
         if scales is None:
-            scales = _new(x, (hidden + 127) // 128, rows, torch.float32)
+            scales = _new(x, ((hidden + 127) // 128, rows), torch.float32, stream)
         p.scales = _operand(scales, "scales", ((hidden + 127) // 128, rows), _ONLY_F32, dev)
     elif scales is not None:
         raise ValueError("scales go with a torch.float8_e4m3fn output")
-    p.rows, p.hidden, p.x_dtype, p.out_dtype = rows, hidden, _DT_WIDE[x.dtype], E4M3 if fp8 else _DT_WIDE[out.dtype]
+    p.rows, p.hidden = rows, _i32(hidden, "hidden")
+    p.x_dtype, p.out_dtype = _DT_WIDE[x.dtype], E4M3 if fp8 else _DT_WIDE[out.dtype]
     p.eps = eps
     check(lib().cottus_rms_norm(C.byref(p), _raw_stream(stream, dev)))
     return (out, scales) if fp8 else out
@@ -366,14 +380,14 @@ def quantize_fp8(x, *, block_rows=1, out=None, scales=None, stream=None):
     p = QuantizeParams()
     p.x = _operand(x, "x", x.shape, _DT_WIDE, dev)
     if out is None:
-        out = torch.empty_like(x, dtype=_FP8)
+        out = _new(x, (rows, cols), _FP8, stream)
     groups = (cols + 127) // 128
     shape = ((rows + 127) // 128, groups) if block_rows == 128 else (groups, rows)
     if scales is None:
-        scales = _new(x, *shape, torch.float32)
+        scales = _new(x, shape, torch.float32, stream)
     p.out = _operand(out, "out", x.shape, _ONLY_FP8, dev)
     p.scales = _operand(scales, "scales", shape, _ONLY_F32, dev)
-    p.rows, p.cols, p.x_dtype, p.block_rows = rows, cols, _DT_WIDE[x.dtype], block_rows
+    p.rows, p.cols, p.x_dtype, p.block_rows = rows, _i32(cols, "cols"), _DT_WIDE[x.dtype], _i32(block_rows, "block_rows")
     check(lib().cottus_quantize_fp8(C.byref(p), _raw_stream(stream, dev)))
     return out, scales
 
@@ -397,9 +411,10 @@ def fp8_linear(x, x_scales, weight, weight_scales, *, residual=None, out=None, o
     if residual is not None:
         p.residual = _operand(residual, "residual", (rows, fout), _ONLY_F32, dev)
     if out is None:
-        out = _new(x, rows, fout, out_dtype)
+        out = _new(x, (rows, fout), out_dtype, stream)
     p.out = _operand(out, "out", (rows, fout), _DT_WIDE, dev)
-    p.rows, p.out_features, p.in_features, p.out_dtype = rows, fout, fin, _DT_WIDE[out.dtype]
+    p.rows, p.out_features, p.in_features = _i32(rows, "rows"), _i32(fout, "out"), _i32(fin, "in")
+    p.out_dtype = _DT_WIDE[out.dtype]
     if status is not None:
         p.status = _operand(status, "status", (1,), _ONLY_I32, dev)
     check(lib().cottus_fp8_linear(C.byref(p), _raw_stream(stream, dev)))
@@ -430,15 +445,15 @@ def sample_tokens(logits, uniforms, *, temperature=None, top_k=None, top_p=None,
     if min_p is not None:
         p.min_p = _operand(min_p, "min_p", row, _ONLY_F32, dev)
     if out is None:
-        out = torch.empty_like(uniforms, dtype=torch.int32)
+        out = _new(logits, row, torch.int32, stream)
     p.tokens = _operand(out, "out", row, _ONLY_I32, dev)
     if return_logprobs and logprobs is None:
-        logprobs = torch.empty_like(uniforms)
+        logprobs = _new(logits, row, torch.float32, stream)
     if logprobs is not None:
         p.logprobs = _operand(logprobs, "logprobs", row, _ONLY_F32, dev)
     if status is not None:
         p.status = _operand(status, "status", (1,), _ONLY_I32, dev)
-    p.batch, p.vocab, p.dtype = batch, vocab, _DT_WIDE[logits.dtype]
+    p.batch, p.vocab, p.dtype = _i32(batch, "batch"), _i32(vocab, "vocab"), _DT_WIDE[logits.dtype]
     check(lib().cottus_sample_tokens(C.byref(p), _raw_stream(stream, dev)))
     return (out, logprobs) if return_logprobs else out
 
@@ -452,7 +467,12 @@ def attention_block_fp8(batch, residual, norm_weight, w_qkv, qkv_scales, w_o, o_
 
     residual [n][hidden] fp32 (updated), w_qkv [(H + 2 Hkv) D][hidden] and w_o [hidden][H D] e4m3 with the scales of
     quantize_fp8(block_rows=128); H D and Hkv D multiples of 128 (a range starts at a scale block).  Returns the
-    attention output [n][H D] fp16."""
+    attention output [n][H D] fp16.  Blocks of different batches may run on different streams at once."""
+    if stream is not None:  # (what is allocated below belongs to the stream that writes it)
+        with torch.cuda.stream(stream):
+            return attention_block_fp8(batch, residual, norm_weight, w_qkv, qkv_scales, w_o, o_scales, kv_pool, cos_sin,
+                                       num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, eps=eps,
+                                       num_layers=num_layers, layer=layer, status=status)
     n, qd, kd = len(batch), num_heads * head_dim, num_kv_heads * head_dim
     if residual.shape[0] != n:
         raise ValueError(f"residual needs one row per active sequence ({n})")
@@ -460,17 +480,16 @@ def attention_block_fp8(batch, residual, norm_weight, w_qkv, qkv_scales, w_o, o_
         raise ValueError("num_heads * head_dim and num_kv_heads * head_dim must be multiples of 128")
     if w_qkv.shape[0] != qd + 2 * kd:
         raise ValueError(f"w_qkv must have {qd + 2 * kd} rows")
-    h, hs = rms_norm(residual, norm_weight, eps=eps, out_dtype=_FP8, stream=stream)
+    h, hs = rms_norm(residual, norm_weight, eps=eps, out_dtype=_FP8)
     qkv = []
     for r0, rows, heads in ((0, qd, num_heads), (qd, kd, num_kv_heads), (qd + kd, kd, num_kv_heads)):
-        part = fp8_linear(h, hs, w_qkv[r0:r0 + rows], qkv_scales[r0 // 128:(r0 + rows) // 128], status=status,
-                          stream=stream)
+        part = fp8_linear(h, hs, w_qkv[r0:r0 + rows], qkv_scales[r0 // 128:(r0 + rows) // 128], status=status)
         qkv.append(part.view(n, heads, head_dim))
     att = rope_append_decode(*qkv, batch.positions[:n], cos_sin, kv_pool, batch.block_table[:n],
                              num_kv_heads=num_kv_heads, head_dim=head_dim, block_size=batch.block_size,
-                             num_layers=num_layers, layer=layer, status=status, stream=stream).view(n, qd)
-    a, a_scales = quantize_fp8(att, stream=stream)
-    fp8_linear(a, a_scales, w_o, o_scales, residual=residual, out=residual, status=status, stream=stream)
+                             num_layers=num_layers, layer=layer, status=status, workspace_of=batch).view(n, qd)
+    a, a_scales = quantize_fp8(att)
+    fp8_linear(a, a_scales, w_o, o_scales, residual=residual, out=residual, status=status)
     return att
 
 
@@ -559,6 +578,17 @@ class DecodeBatch:
         self._h = h
         self.num_blocks, self.block_size = num_blocks, block_size
         self.max_batch, self.max_blocks_per_seq = max_batch, max_blocks_per_seq
+        self._workspaces = []  # (all of them: a captured graph may hold an earlier, smaller one)
+
+    def workspace(self, nbytes: int) -> torch.Tensor:
+        """This batch's scratch buffer for the decode kernels (whose counter words are zero between calls).  While a
+        graph is captured a buffer that does not exist yet is the graph's own, cleared at each replay."""
+        if self._workspaces and self._workspaces[-1].numel() >= nbytes:
+            return self._workspaces[-1]
+        buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=self.positions.device)
+        if not torch.cuda.is_current_stream_capturing():
+            self._workspaces.append(buf)
+        return buf
 
     def add(self, seq_id: int) -> int:
         row = C.c_int32()

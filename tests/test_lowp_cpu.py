@@ -138,3 +138,25 @@ def test_host_tensors_are_refused():
     x = torch.zeros(2, 128)
     with pytest.raises(ValueError):
         cb.rms_norm(x, torch.ones(128))
+
+
+WIDE = (1 << 30) + 16
+
+
+@pytest.mark.parametrize("call", [lambda: _norm(rows=1, hidden=WIDE), lambda: _norm(rows=1, hidden=(1 << 31) - 8),
+                                  lambda: _quant(rows=1, cols=WIDE), lambda: _quant(rows=1, cols=(1 << 31) - 1, block_rows=128),
+                                  lambda: _quant(rows=(1 << 63) - 1, cols=1, block_rows=128, x=1 << 60),
+                                  lambda: _linear(rows=WIDE, in_features=16), lambda: _linear(rows=1, out_features=(1 << 31) - 1),
+                                  lambda: _linear(rows=1, in_features=WIDE)])
+def test_sizes_that_32_bit_columns_cannot_round_up(call):
+    assert call() == UNSUP
+    assert "too" in _message()
+
+
+def test_sizes_past_32_bits_are_not_cut():
+    """ctypes keeps the lower 32 bits of a larger size; the wrappers refuse it."""
+    from cottus_b200 import ops
+    assert ops._i32((1 << 31) - 1, "rows") == (1 << 31) - 1
+    for n in (1 << 31, (1 << 32) + 5, -1):
+        with pytest.raises(ValueError, match="rows"):
+            ops._i32(n, "rows")

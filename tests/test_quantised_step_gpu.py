@@ -7,6 +7,11 @@ The blocks are compositions: their results equal, bit for bit, those of the
 operators called one by one (each is held to its definition elsewhere), and
 their attention is held to the oracle from the projections on.
 """
+import os
+import pathlib
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -201,3 +206,98 @@ def test_weights_written_just_before():
     torch.cuda.synchronize()
     for i, o in enumerate(outs):
         assert torch.equal(o, want[i % 3]), i
+
+
+def _long_batches(n, tokens):
+    """Batches of one long sequence each, with room for what their split decode needs."""
+    out = []
+    for i in range(n):
+        b = cb.DecodeBatch(tokens // BS + 2, BS, 1, tokens // BS + 2, device=DEV)
+        b.add(i)
+        for _ in range(tokens):
+            b.begin_step()
+            b.end_step()
+        b.begin_step()
+        out.append(b)
+    torch.cuda.synchronize()
+    return out
+
+
+def test_blocks_of_two_batches_at_once():
+    """Two batches with a long context each, on two streams, by the stream argument, and captured as the first call of
+    their batch: each has its own workspace and its temporaries from its own stream's pool."""
+    tokens = 1500
+    layers, _, _ = _weights(7)
+    tab = cb.rope_cos_sin_table(tokens + BS, D).to(DEV)
+    g = torch.Generator(device=DEV).manual_seed(8)
+    pools, want, start = [], [], []
+    batches = _long_batches(2, tokens)
+    for b in batches:
+        pools.append(torch.randn(b.num_blocks * 2 * LAYERS * BS * HKV * D, generator=g, device=DEV).half().view(torch.int16))
+        start.append(torch.randn(1, HIDDEN, generator=g, device=DEV))
+        r = start[-1].clone()
+        att = [_block(b, r, w, pools[-1], tab, i) for i, w in enumerate(layers)]
+        want.append((att, r))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    rows = [[s.clone() for _ in range(20)] for s in start]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for j in range(20):
+        for i, s in enumerate(streams):
+            for layer, w in enumerate(layers):
+                got[i].append(cb.attention_block_fp8(batches[i], rows[i][j], w["norm"], *w["qkv"], *w["o"], pools[i], tab,
+                                                     num_heads=H, num_kv_heads=HKV, head_dim=D, num_layers=LAYERS, layer=layer,
+                                                     stream=s))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for j in range(20):
+            assert torch.equal(rows[i][j], want[i][1])
+            for layer in range(LAYERS):
+                assert torch.equal(got[i][j * LAYERS + layer], want[i][0][layer])
+    # captured before their batch ever ran eagerly
+    graphs = []
+    for i, b in enumerate(_long_batches(2, tokens)):
+        r = start[i].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for layer, w in enumerate(layers):
+                _block(b, r, w, pools[i], tab, layer)
+        graphs.append((graph, r, b))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for i, (graph, r, _) in enumerate(graphs):
+            with torch.cuda.stream(streams[i]):
+                r.copy_(start[i])
+                graph.replay()
+    torch.cuda.synchronize()
+    for i, (_, r, _) in enumerate(graphs):
+        assert torch.equal(r, want[i][1])
+
+
+def test_first_call_inside_a_capture():
+    """A process whose first call of each operator is captured: what a call sets up once is no stream work."""
+    script = """
+import torch, cottus_b200 as cb
+dev = "cuda"
+r, u = torch.randn(3, 256, device=dev), torch.rand(3, device=dev)
+n = torch.ones(256, device=dev)
+wide = torch.randn(300, 256, device=dev)
+p = torch.full((3,), 0.9, device=dev)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    w, ws = cb.quantize_fp8(torch.ones(5000, 256, device=dev) * u[0] + n, block_rows=128)
+    x, xs = cb.quantize_fp8(wide)
+    y = cb.fp8_linear(x, xs, w, ws)
+    t, logits = cb.next_tokens(r, n, w, ws, u, top_p=p)
+g.replay()
+torch.cuda.synchronize()
+t2, l2 = cb.next_tokens(r, n, w, ws, u, top_p=p)
+assert torch.equal(t, t2) and torch.equal(logits, l2) and torch.equal(y, cb.fp8_linear(x, xs, w, ws))
+print("same")
+"""
+    root = pathlib.Path(cb.__file__).resolve().parents[1]
+    out = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300,
+                         env={**os.environ, "PYTHONPATH": str(root)})
+    assert out.returncode == 0 and "same" in out.stdout, out.stderr[-2000:]
