@@ -84,6 +84,35 @@ def test_against_64_bits(m, n, k, out_dtype, residual):
     _check(got, x, xs, w, ws, res)
 
 
+# around the borders between the tiles: rows of x, a ring shorter than the groups of one CTA, every number of splits,
+# the wide tile with rows that its stores cannot take whole
+BORDERS = [(m, n, k) for m in (2, 15, 17, 31, 32, 33, 63, 65, 96) for n, k in ((260, 1040), (20001, 2064))] + \
+    [(16, 128 * t, 1152) for t in (1, 13, 18, 22, 29, 37, 49, 73, 74, 100, 148, 149)] + \
+    [(900, 3001, 400), (513, 9000, 16), (257, 10001, 128)]
+
+
+@pytest.mark.parametrize("m, n, k", BORDERS)
+def test_tile_borders(m, n, k):
+    x, xs, w, ws = _quantised(m, n, k, m + n + k)
+    res = torch.randn(m, n, generator=torch.Generator().manual_seed(n))
+    dev = [t.to(DEV) for t in (x, xs, w, ws)]
+    _check(cb.fp8_linear(*dev), x, xs, w, ws, None)
+    _check(cb.fp8_linear(*dev, residual=res.to(DEV), out_dtype=torch.float32), x, xs, w, ws, res)
+
+
+def test_elements_past_32_bits():
+    """More than 2^31 results: the last rows equal those of a call of their own (the same tiles)."""
+    m, n, k, last = 40000, 56000, 128, 2000
+    g = torch.Generator(device=DEV).manual_seed(12)
+    x, xs = cb.quantize_fp8(torch.randn(m, k, generator=g, device=DEV))
+    w, ws = cb.quantize_fp8(torch.randn(n, k, generator=g, device=DEV), block_rows=128)
+    y = cb.fp8_linear(x, xs, w, ws)
+    tail = cb.fp8_linear(x[-last:], xs[:, -last:].contiguous(), w, ws)
+    assert y.numel() > 1 << 31 and torch.equal(y[-last:], tail)
+    head = cb.fp8_linear(x[:last], xs[:, :last].contiguous(), w, ws)
+    assert torch.equal(y[:last], head)
+
+
 def test_long_sums_keep_32_bits():
     """Products of 2^16 and of 2^-6 in one group: the sum needs 23 bits, so a narrower accumulator shows."""
     x = torch.full((4, 128), 2.0 ** -3)

@@ -186,6 +186,27 @@ def test_quantize_writes_its_rows_only():
     assert torch.all(buf[:136] == 0x55) and torch.all(buf[6 * 136:] == 0x55) and torch.all(sc.view(-1)[10:] == 3.0)
 
 
+def test_elements_past_32_bits():
+    """More than 2^31 elements: the last rows equal those of a call of their own."""
+    rows, cols, last = 300000, 7200, 700
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=DEV)
+    x[:1000].normal_()
+    x[1000:] = x[:1000].repeat(299, 1)
+    x[-last:].normal_()
+    assert x.numel() > 1 << 31
+    w = torch.randn(cols, device=DEV)
+    assert torch.equal(cb.rms_norm(x, w)[-last:], cb.rms_norm(x[-last:], w))
+    q, s = cb.rms_norm(x, w, out_dtype=FP8)
+    q1, s1 = cb.rms_norm(x[-last:], w, out_dtype=FP8)
+    assert torch.equal(q[-last:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[:, -last:], s1)
+    q, s = cb.quantize_fp8(x)
+    q1, s1 = cb.quantize_fp8(x[-last:])
+    assert torch.equal(q[-last:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[:, -last:], s1)
+    q, s = cb.quantize_fp8(x, block_rows=128)
+    q1, s1 = cb.quantize_fp8(x[rows // 128 * 128 - 256:], block_rows=128)
+    assert torch.equal(q[rows // 128 * 128 - 256:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[-3:], s1)
+
+
 def test_refusals():
     x, w = torch.zeros(2, 256, device=DEV), torch.ones(256, device=DEV)
     with pytest.raises(ValueError, match="contiguous"):

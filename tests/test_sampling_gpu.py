@@ -178,6 +178,22 @@ def test_largest_vocabulary():
             assert int(tok[b]) == want and abs(float(lp[b]) - wlp) <= abs(wlp) * 2.0 ** -24 + 2e-8
 
 
+def test_logits_past_32_bits():
+    """More than 2^31 logits: the last rows' tokens equal those of a call of their own, filter by filter."""
+    batch, vocab, last = 17000, 128256, 160
+    logits = torch.empty(batch, vocab, dtype=torch.float16, device=DEV)
+    logits[:500].normal_()
+    logits[500:] = logits[:500].repeat(33, 1)
+    logits[-last:].normal_()
+    assert logits.numel() > 1 << 31
+    u = torch.rand(batch, device=DEV)
+    p, k = torch.full((batch,), 0.7, device=DEV), torch.full((batch,), 30, dtype=torch.int32, device=DEV)
+    for kw in (dict(), dict(top_p=p), dict(top_k=k, top_p=p)):
+        got = cb.sample_tokens(logits, u, **kw)
+        part = cb.sample_tokens(logits[-last:], u[-last:], **{n: t[-last:] for n, t in kw.items()})
+        assert torch.equal(got[-last:], part)
+
+
 def test_writes_its_rows_only_and_refuses():
     x, u = _logits(3, 100, torch.float32, 1)
     x, u = x.to(DEV), u.to(DEV)
