@@ -17,7 +17,9 @@
 //      which the count or the mass passes its target; its few members are
 //      gathered by the first CTA, sorted by key, and the threshold is read
 //      off their prefix sums.  A bin with more members than the list holds is
-//      first split by histograms of the key itself;
+//      first split by histograms of the key itself.  top_k up to 1024, and
+//      top-p alone, start from a histogram of counts (an atomic per logit
+//      where count and mass take four);
 //   3. the kept mass per warp, each warp owning a contiguous run of indices,
 //      then the one warp whose run holds uniform * mass walks it.
 //
@@ -79,7 +81,7 @@ constexpr int kTable = 256;    // 2^(j/256)
 
 // Shared memory behind the slice.
 struct Shared {
-    u64 exp2_table[kTable];  // with one bit more than the weights
+    u64 exp2_table[kTable];  // with 14 bits more than the weights
     uint32_t count[kBins];  // histogram: members,
     uint32_t limb[3][kBins];  // and their mass in limbs of limb_bits
     u64 list[kList];
@@ -192,24 +194,44 @@ struct Weight {
         return v < -(frac + 2) * 0.6931471805599453 ? 0 : __double2ull_rn(exp(v) * unit());
     }
     __device__ __forceinline__ u64 operator()(float x) const { return plain ? fast(x) : general(x); }
-    // (0 for -inf and NaN)
-    __device__ __forceinline__ u64 fast(float x) const {
+    __device__ __forceinline__ u64 fast(float x) const { return fast(x, x).x; }
+    // Of two logits (0 for -inf and NaN).  The arithmetic of both is packed, and
+    // what is integer kept short: that pipe has half the rate, and bounds the
+    // passes over all logits (25 such operations per logit before: 256 x 50257
+    // fp16 without filters 44 us, so 38).
+    struct Pair {
+        u64 x, y;
+    };
+    __device__ __forceinline__ Pair fast(float x0, float x1) const {
+        constexpr float magic = 12582912.f;  // 1.5 2^23: a float above it holds an integer in its low bits
+        const float2 x = make_float2(x0, x1), one = make_float2(1.f, 1.f), minus = make_float2(-1.f, -1.f);
+        const float2 tops = make_float2(top, top);
         // x - top = d + e exactly
-        const float d = x - top, b = d - x, e = (x - (d - b)) - (top + b);
-        const float y = d * c;
-        const float yl = fmaf(e, c, fmaf(d, cl, fmaf(d, c, -y)));
-        // m = rint(256 y): the low bits of y 256 + 1.5 2^23
-        const float magic = 12582912.f;
-        const float t = fmaf(y, 256.f, magic);
-        const int m = __float_as_int(t) - __float_as_int(magic);
-        const float r = fmaf(t - magic, -1.f / 256.f, y) + yl;
-        // 2^r - 1 = sum (r ln 2)^i / i!
-        const float q = r * fmaf(r, fmaf(r, 0.0555041087f, 0.240226507f), 0.693147181f);
-        const int qi = __float_as_int(fmaf(q, 2147483648.f, magic)) - __float_as_int(magic);
-        const u64 p = table[m & (kTable - 1)];
-        const u64 v = p + (u64)(((long long)(int)(p >> 18) * qi) >> 13);  // p < 2^49
-        const int sh = -(m >> 8) & 63;
-        return y > -(float)(frac + 2) ? ((v >> sh) + 1) >> 1 : 0;
+        const float2 d = ffma2(tops, minus, x), b = ffma2(x, minus, d);
+        const float2 e = ffma2(ffma2(b, one, tops), minus, ffma2(ffma2(b, minus, d), minus, x));
+        // -y = -(d c) and what it leaves out
+        const float2 cc = make_float2(c, c), ny = fmul2(d, make_float2(-c, -c));
+        const float2 yl = ffma2(e, cc, ffma2(d, make_float2(cl, cl), ffma2(d, cc, ny)));
+        // m = rint(256 y); from y = -64 on (or NaN) the shift below leaves nothing
+        const float2 t = ffma2(make_float2(fminf(ny.x, 64.f), fminf(ny.y, 64.f)), make_float2(-256.f, -256.f),
+                               make_float2(magic, magic));
+        const float2 m = ffma2(t, one, make_float2(-magic, -magic));
+        const float2 r = ffma2(ffma2(m, make_float2(1.f / 256.f, 1.f / 256.f), ny), minus, yl);
+        // 2^r - 1 = sum (r ln 2)^i / i!, in units of 2^-31
+        const float2 q = fmul2(r, ffma2(r, ffma2(r, make_float2(0.0555041087f, 0.0555041087f), make_float2(0.240226507f, 0.240226507f)),
+                                        make_float2(0.693147181f, 0.693147181f)));
+        const float2 qs = ffma2(q, make_float2(2147483648.f, 2147483648.f), make_float2(magic, magic));
+        return {scaled(t.x, qs.x), scaled(t.y, qs.y)};
+    }
+    // 2^(m / 256) (1 + q) from the floats that hold m and q.
+    __device__ __forceinline__ u64 scaled(float t, float qs) const {
+        constexpr uint32_t magic = 0x4B400000u;
+        const uint32_t m = __float_as_uint(t);
+        const u64 p = table[m & (kTable - 1)];  // below 2^62, 13 bits more than 2^(j/256) has
+        const u64 v = p + (u64)((long long)(int)(p >> 31) * (int)(__float_as_uint(qs) - magic));
+        u64 w;  // (a shift by 64 or more is 0)
+        asm("shr.u64 %0, %1, %2;" : "=l"(w) : "l"(v), "r"((14 + (magic >> 8)) - (m >> 8)));
+        return w;
     }
 };
 
@@ -274,8 +296,10 @@ struct Row {
         }
     }
     // Adds the cluster's histograms up, every CTA for itself, into its mcnt /
-    // mmass (16 loads of four bins per thread, all in flight).  The
-    // histogram may be cleared, or its words used, after the next cluster barrier.
+    // mmass (four bins per thread).  The histogram may be cleared, or its words
+    // used, after the next cluster barrier.  (Code that runs once costs its
+    // way through the instruction caches first: with the loads of all CTAs
+    // unrolled this took 20k cycles, so 10k.)
     __device__ void merge_hist() const {
         csync();
         constexpr int Q = kBins / 4;  // runs of four bins
@@ -284,17 +308,12 @@ struct Row {
         const bool low = threadIdx.x < Q;
         const uint32_t* a0 = low ? &s.count[b] : &s.limb[1][b];
         const uint32_t* a1 = low ? &s.limb[0][b] : &s.limb[2][b];
-        uint4 x[kMaxCluster], y[kMaxCluster];
-#pragma unroll
-        for (int q = 0; q < kMaxCluster; ++q) {
-            x[q] = q < size ? ld_cluster_u4(mapa(a0, q)) : make_uint4(0, 0, 0, 0);
-            y[q] = q < size ? ld_cluster_u4(mapa(a1, q)) : make_uint4(0, 0, 0, 0);
-        }
         u64 cx[4] = {0, 0, 0, 0}, cy[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int q = 0; q < kMaxCluster; ++q) {
-            cx[0] += x[q].x, cx[1] += x[q].y, cx[2] += x[q].z, cx[3] += x[q].w;
-            cy[0] += y[q].x, cy[1] += y[q].y, cy[2] += y[q].z, cy[3] += y[q].w;
+#pragma unroll 2
+        for (int q = 0; q < size; ++q) {
+            const uint4 x = ld_cluster_u4(mapa(a0, q)), y = ld_cluster_u4(mapa(a1, q));
+            cx[0] += x.x, cx[1] += x.y, cx[2] += x.z, cx[3] += x.w;
+            cy[0] += y.x, cy[1] += y.y, cy[2] += y.z, cy[3] += y.w;
         }
         if (low) {
 #pragma unroll
@@ -345,14 +364,10 @@ struct Row {
             s.pick_mass = 0;
         }
         __syncthreads();
-        cb -= ctot;
-        mb += mass0 - mtot;
-#pragma unroll
-        for (int w = 0; w < kW; ++w)
-            if (w < warp) {
-                cb += s.wcnt[w];
-                mb += s.wsum[w];
-            }
+        const uint32_t cw = s.wcnt[lane % kW];
+        const u64 mw = s.wsum[lane % kW];
+        cb += __shfl_sync(0xffffffffu, warp_scan(cw, lane) - cw, warp) - ctot;
+        mb += __shfl_sync(0xffffffffu, warp_scan(mw, lane) - mw, warp) - mtot + mass0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             // sums only grow, so one bin takes them past the target
@@ -370,6 +385,53 @@ struct Row {
         return {(int)s.pick_bin, s.pick_cnt, s.pick_in, s.pick_mass};
     }
 
+    // Every CTA's count of each distance, added up by every CTA for itself into
+    // its mcnt.  with_mass: mmass gets what the counts say of the masses, a
+    // token weighing what the middle of its bin weighs (the maximum itself 1).
+    __device__ void count_distances(bool with_mass) const {
+        each([&](float v, int) { atomicAdd(&s.count[distance_bin(weight.top, v)], 1u); });
+        csync();
+#pragma unroll 1
+        for (int b = threadIdx.x; b < kBins; b += kT) {
+            uint32_t sum = 0;
+#pragma unroll 4
+            for (int q = 0; q < size; ++q) sum += ld_cluster(mapa(&s.count[b], q));
+            s.mcnt[b] = sum;
+            u64 m = 0;
+            if (with_mass) {
+                const float mid = b == 0 ? 0.125f : (b == kBins - 1 ? near_edge(b) : 0.5f * (near_edge(b) + far_edge(b)));
+                const u64 w = weight.fast(weight.top - mid);
+                m = b == 0 ? (u64)(sum - 1) * w + (1ull << weight.frac) : sum * w;
+            }
+            s.mmass[b] = m;
+        }
+        __syncthreads();
+    }
+    // The bins in which the running mass reaches (p - eps) and (p + eps) times
+    // its end (0 and the last one, where it never does).
+    __device__ void mass_range(float p, float eps, int& lo, int& hi) const {
+        constexpr int PER = kBins / kT;
+        u64 m[PER], own = 0, total;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) own += m[j] = s.mmass[threadIdx.x * PER + j];
+        if (threadIdx.x == 0) {
+            s.pick_bin = 0;
+            s.pick_in = kBins - 1;
+        }
+        u64 run = block_before(own, total);
+        const double t0 = ((double)p - eps) * (double)total, t1 = ((double)p + eps) * (double)total;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const double a = (double)run, b = (double)(run + m[j]);
+            if (a < t0 && b >= t0) s.pick_bin = threadIdx.x * PER + j;
+            if (a < t1 && b >= t1) s.pick_in = threadIdx.x * PER + j;
+            run += m[j];
+        }
+        __syncthreads();
+        lo = (int)s.pick_bin;
+        hi = (int)s.pick_in;
+    }
+
     // Level one: the histogram of the distance to the maximum.
     __device__ void build_l1(bool mass) const {
         clear_hist();
@@ -384,6 +446,7 @@ struct Row {
         if ((threadIdx.x & 31) == 0) s.wsum[threadIdx.x >> 5] = m;
         __syncthreads();
         m = 0;
+#pragma unroll 1
         for (int w = 0; w < kW; ++w) m += s.wsum[w];
         __syncthreads();
         return m;
@@ -522,8 +585,7 @@ struct Row {
         __syncthreads();
         if ((threadIdx.x & 31) == 0) s.wsum[threadIdx.x >> 5] = v;
         __syncthreads();
-        for (int w = 0; w < kW; ++w) v = s.wsum[w] < v ? s.wsum[w] : v;
-        return v;
+        return warp_min(s.wsum[threadIdx.x % kW]);
     }
     // Sum of `own` over the threads before this one; `total` over all.
     __device__ u64 block_before(u64 own, u64& total) const {
@@ -532,13 +594,9 @@ struct Row {
         __syncthreads();  // (earlier readers of wsum are done)
         if (lane == 31) s.wsum[warp] = incl;
         __syncthreads();
-        u64 before = incl - own;
-        total = 0;
-        for (int w = 0; w < kW; ++w) {
-            if (w < warp) before += s.wsum[w];
-            total += s.wsum[w];
-        }
-        return before;
+        const u64 upto = warp_scan(s.wsum[lane % kW], lane);  // (in lanes below kW)
+        total = __shfl_sync(0xffffffffu, upto, kW - 1);
+        return __shfl_sync(0xffffffffu, upto, warp) - s.wsum[warp] + incl - own;
     }
     // Smallest value of the block's threads, in every thread.
     __device__ uint32_t block_min(uint32_t v) const {
@@ -558,25 +616,21 @@ struct Row {
         if (m > top_k) m = top_k;
         constexpr int PER = kList / kT;
         const int per = (m + kT - 1) / kT, at = threadIdx.x * per;  // this thread's run of entries
-        u64 w[PER], own = 0, total;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            w[j] = j < per && at + j < m ? weight(from_desc((uint32_t)(s.list[at + j] >> 32))) : 0;
-            own += w[j];
-        }
+        u64 own = 0, total;
+#pragma unroll 1
+        for (int i = at; i < at + per && i < m; ++i) own += weight(from_desc((uint32_t)(s.list[i] >> 32)));
         u64 run = block_before(own, total);
         // entries that stay: up to the one at which the mass reaches its
         // share, and with at least the least weight; both cut the order off
         const double t = (double)top_p * (double)total;
         const u64 least = min_p > 0.f ? __double2ull_ru((double)min_p * weight.unit()) : 0;
         uint32_t cut = (uint32_t)m;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            run += w[j];
-            if (j < per && at + j < m) {
-                if (w[j] < least) cut = min(cut, (uint32_t)(at + j));
-                if (top_p < 1.f && (double)run >= t) cut = min(cut, (uint32_t)(at + j + 1));
-            }
+#pragma unroll 1
+        for (int i = at; i < at + per && i < m; ++i) {
+            const u64 w = weight(from_desc((uint32_t)(s.list[i] >> 32)));
+            run += w;
+            if (w < least) cut = min(cut, (uint32_t)i);
+            if (top_p < 1.f && (double)run >= t) cut = min(cut, (uint32_t)(i + 1));
         }
         const int kept = (int)block_min(cut);
         // the draw, in index order: (index, logit) keys, sorted
@@ -593,23 +647,19 @@ struct Row {
         __syncthreads();
         sort_list(kept);
         own = 0;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            w[j] = j < per && at + j < kept ? weight(from_desc((uint32_t)s.list[at + j])) : 0;
-            own += w[j];
-        }
+#pragma unroll 1
+        for (int i = at; i < at + per && i < kept; ++i) own += weight(from_desc((uint32_t)s.list[i]));
         run = block_before(own, total);
         const double draw = (double)u * (double)total;
         if ((double)(run + own) > draw && !((double)run > draw)) {
-            bool found = false;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                run += w[j];
-                if (!found && (double)run > draw) {
-                    found = true;
-                    *token = (int32_t)(s.list[at + j] >> 32);
-                    if (logprob)
-                        *logprob = (float)(weight.z(from_desc((uint32_t)s.list[at + j])) - log((double)total / weight.unit()));
+#pragma unroll 1
+            for (int i = at;; ++i) {
+                const float x = from_desc((uint32_t)s.list[i]);
+                run += weight(x);
+                if ((double)run > draw) {
+                    *token = (int32_t)(s.list[i] >> 32);
+                    if (logprob) *logprob = (float)(weight.z(x) - log((double)total / weight.unit()));
+                    break;
                 }
             }
         }
@@ -617,22 +667,97 @@ struct Row {
 
     // The threshold key at which the running count reaches k, or the running
     // mass reaches t, among the keys up to `limit`; `limit` where it does not.
+    // gathered: the lists hold the keys among which it does, behind mass_to.
     // l1: the merged arrays hold the level-one histogram (with masses, where
     // need_mass); false on return if they no longer do.  mass_to (need_mass):
     // the mass of everything up to the threshold.
-    __device__ __forceinline__ u64 select(bool by_mass, uint32_t k, double t, u64 limit, bool need_mass, bool& l1, u64& mass_to) const {
+    __device__ __forceinline__ u64 select(bool by_mass, uint32_t k, double t, u64 limit, bool need_mass, bool gathered, bool& l1,
+                                          u64& mass_to) const {
+        uint32_t before_cnt = 0;
+        u64 before_mass = mass_to;
+        if (!gathered && !gather(by_mass, k, t, limit, need_mass, l1, before_cnt, before_mass)) {
+            mass_to = before_mass;
+            return limit;
+        }
+        csync();
+        if (rank == 0) {
+            int m = collect_lists();
+            while (m > kCountSort) m = narrow_list(m, by_mass, k, t, before_cnt, before_mass, need_mass);
+            sort_list(m);
+            // prefix masses of the sorted members, in runs of `per` per thread
+            const int per = (m + kT - 1) / kT;
+            const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+            u64 own = 0;
+            if (need_mass)
+#pragma unroll 1
+                for (int j = 0; j < per; ++j) {
+                    const int i = threadIdx.x * per + j;
+                    if (i < m) own += weight(from_desc((uint32_t)(s.list[i] >> 32)));
+                }
+            const u64 incl = warp_scan(own, lane);
+            if (lane == 31) s.wsum[warp] = incl;
+            if (threadIdx.x == 0) s.pick_bin = 0x7fffffffu;
+            __syncthreads();
+            u64 run = before_mass + incl - own;
+#pragma unroll 1
+            for (int w = 0; w < warp; ++w) run += s.wsum[w];
+            const u64 run0 = run;
+#pragma unroll 1
+            for (int j = 0; j < per; ++j) {
+                const int i = threadIdx.x * per + j;
+                if (i >= m) break;
+                if (need_mass) run += weight(from_desc((uint32_t)(s.list[i] >> 32)));
+                const bool hit = i == m - 1 || (by_mass ? (double)run >= t : before_cnt + (uint32_t)i + 1 >= k);
+                if (hit) {
+                    atomicMin(&s.pick_bin, (uint32_t)i);
+                    break;
+                }
+            }
+            __syncthreads();
+            const int hit = (int)s.pick_bin;
+            if (m == 0) {  // (a picked bin has members)
+                if (threadIdx.x < size) {
+                    st_cluster(mapa(&s.res[0], threadIdx.x), limit);
+                    st_cluster(mapa(&s.res[1], threadIdx.x), before_mass);
+                }
+            } else if (threadIdx.x == hit / per) {
+                u64 r = run0;
+                if (need_mass)
+#pragma unroll 1
+                    for (int i = threadIdx.x * per; i <= hit; ++i)
+                        r += weight(from_desc((uint32_t)(s.list[i] >> 32)));
+                const u64 key = s.list[hit];
+#pragma unroll 1
+                for (int q = 0; q < size; ++q) {
+                    st_cluster(mapa(&s.res[0], q), key);
+                    st_cluster(mapa(&s.res[1], q), r);
+                }
+            }
+        }
+        csync();
+        l1 = false;  // (the first CTA's merged words may have served its list)
+        mass_to = s.res[1];
+        const u64 thr = s.res[0];
+        __syncthreads();
+        return thr;
+    }
+
+    // select's first part: the members of the bin of the threshold into the
+    // lists; false (with the mass of all candidates) where none is reached.
+    __device__ __forceinline__ bool gather(bool by_mass, uint32_t k, double t, u64 limit, bool need_mass, bool& l1,
+                                           uint32_t& before_cnt, u64& before_mass) const {
         if (!l1) build_l1(need_mass);
         l1 = true;
         Pick p = pick_bin(by_mass, k, 0, t);
         if (p.bin == kBins) {  // fewer candidates than k
-            mass_to = need_mass ? l1_mass() : 0;
-            return limit;
+            before_mass = need_mass ? l1_mass() : 0;
+            return false;
         }
         const int level_bin = p.bin;
         u64 kmin = 0, kmax = limit;  // members: keys in this range (and, at first, of the picked bin)
         bool by_bin = true;
-        uint32_t before_cnt = p.before_cnt;
-        u64 before_mass = p.before_mass;
+        before_cnt = p.before_cnt;
+        before_mass = p.before_mass;
         auto member = [&](float v, u64 key) {
             return by_bin ? distance_bin(weight.top, v) == level_bin && key <= limit : key >= kmin && key <= kmax;
         };
@@ -674,62 +799,7 @@ struct Row {
             const u64 key = order_key(v, (uint32_t)i);
             if (member(v, key)) s.list[atomicAdd(&s.list_n, 1u)] = key;
         });
-        csync();
-        if (rank == 0) {
-            int m = collect_lists();
-            while (m > kT) m = narrow_list(m, by_mass, k, t, before_cnt, before_mass, need_mass);
-            sort_list(m);
-            // prefix masses of the sorted members, in runs of `per` per thread
-            const int per = (m + kT - 1) / kT;
-            const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-            u64 own = 0;
-            if (need_mass)
-                for (int j = 0; j < per; ++j) {
-                    const int i = threadIdx.x * per + j;
-                    if (i < m) own += weight(from_desc((uint32_t)(s.list[i] >> 32)));
-                }
-            const u64 incl = warp_scan(own, lane);
-            if (lane == 31) s.wsum[warp] = incl;
-            if (threadIdx.x == 0) s.pick_bin = 0x7fffffffu;
-            __syncthreads();
-            u64 run = before_mass + incl - own;
-            for (int w = 0; w < warp; ++w) run += s.wsum[w];
-            const u64 run0 = run;
-            for (int j = 0; j < per; ++j) {
-                const int i = threadIdx.x * per + j;
-                if (i >= m) break;
-                if (need_mass) run += weight(from_desc((uint32_t)(s.list[i] >> 32)));
-                const bool hit = i == m - 1 || (by_mass ? (double)run >= t : before_cnt + (uint32_t)i + 1 >= k);
-                if (hit) {
-                    atomicMin(&s.pick_bin, (uint32_t)i);
-                    break;
-                }
-            }
-            __syncthreads();
-            const int hit = (int)s.pick_bin;
-            if (m == 0) {  // (a picked bin has members)
-                if (threadIdx.x < size) {
-                    st_cluster(mapa(&s.res[0], threadIdx.x), limit);
-                    st_cluster(mapa(&s.res[1], threadIdx.x), before_mass);
-                }
-            } else if (threadIdx.x == hit / per) {
-                u64 r = run0;
-                if (need_mass)
-                    for (int i = threadIdx.x * per; i <= hit; ++i)
-                        r += weight(from_desc((uint32_t)(s.list[i] >> 32)));
-                const u64 key = s.list[hit];
-                for (int q = 0; q < size; ++q) {
-                    st_cluster(mapa(&s.res[0], q), key);
-                    st_cluster(mapa(&s.res[1], q), r);
-                }
-            }
-        }
-        csync();
-        l1 = false;  // (the first CTA's merged words may have served its list)
-        mass_to = s.res[1];
-        const u64 thr = s.res[0];
-        __syncthreads();
-        return thr;
+        return true;
     }
 
     // Smallest v of the cluster's threads, in every thread.  `use` names the
@@ -746,9 +816,7 @@ struct Row {
             if (lane < size) st_cluster(mapa(&s.slot[use][rank], lane), v);
         }
         csync();
-        v = kNoKey;
-        for (int q = 0; q < size; ++q) v = s.slot[use][q] < v ? s.slot[use][q] : v;
-        return v;
+        return warp_min(s.slot[use][lane % size]);
     }
 };
 
@@ -776,7 +844,7 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const SampleArgs a) {
     if (threadIdx.x == 0) s.list_n = 0;
     if (threadIdx.x < kTable) {
         const double unit = (double)(1ull << (a.frac_bits + 1));
-        s.exp2_table[threadIdx.x] = __double2ull_rn(exp2(threadIdx.x * (1.0 / kTable)) * unit);
+        s.exp2_table[threadIdx.x] = __double2ull_rn(exp2(threadIdx.x * (1.0 / kTable)) * unit) << 13;
     }
     grid_dependency_wait();
     grid_dependents_launch();
@@ -838,18 +906,7 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const SampleArgs a) {
         // few candidates: their histogram by count alone, every CTA adding up
         // the cluster's; the first CTA gets all up to the bin in which the
         // count reaches top_k, and does the rest by itself
-        r.each([&](float v, int) { atomicAdd(&s.count[distance_bin(top, v)], 1u); });
-        csync();
-        for (int b = threadIdx.x; b < kBins; b += kT) {
-            uint32_t c[kMaxCluster], sum = 0;  // (all loads in flight together)
-#pragma unroll
-            for (int q = 0; q < kMaxCluster; ++q) c[q] = q < size ? ld_cluster(mapa(&s.count[b], q)) : 0;
-#pragma unroll
-            for (int q = 0; q < kMaxCluster; ++q) sum += c[q];
-            s.mcnt[b] = sum;
-            s.mmass[b] = 0;
-        }
-        __syncthreads();
+        r.count_distances(false);
         const auto p = r.pick_bin(false, (uint32_t)top_k, 0, 0.0);
         if (p.before_cnt + p.in_cnt <= (uint32_t)kList) {  // (no bin picked: top_k candidates or fewer)
             const uint32_t counter = mapa(&s.list_n, 0), list0 = mapa(&s.list[0], 0);
@@ -865,46 +922,140 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const SampleArgs a) {
         }
         csync();  // (the histogram is about to be cleared)
     }
-    // first by count, then by mass
-    bool l1 = false;
-    u64 mass = 0;
-    for (int by_mass = by_k ? 0 : 1; by_mass < (by_p ? 2 : 1); ++by_mass) {
-        if (by_mass && !by_k) {  // the whole mass first: one histogram serves both
-            r.build_l1(true);
-            l1 = true;
-            mass = r.l1_mass();
-        }
-        thr = r.select(by_mass != 0, (uint32_t)top_k, (double)top_p * (double)mass, thr, by_p, l1, mass);
-    }
-
-    // the kept mass: each thread owns a contiguous run of vectors (an odd
-    // number, so that the lanes of a warp read from different banks)
+    // each thread owns a contiguous run of vectors (an odd number, so that the
+    // lanes of a warp read from different banks)
     const int run = (vecs + kT - 1) / kT | 1;
     const int v0 = threadIdx.x * run < vecs ? threadIdx.x * run : vecs, v1 = v0 + run < vecs ? v0 + run : vecs;
     // min-p in the weights' units (0: off, as for NaN; the largest weight, 1, always stays)
     const u64 least_w = min_p > 0.f ? __double2ull_ru((double)min_p * r.weight.unit()) : 0;
-    const bool filtered = thr != kNoKey || least_w > 0 || !r.weight.plain;
+
+    bool near = false;  // the members around top-p's threshold are in the lists
+    u64 mass = 0, own = 0;
+    u64 mine[kList / kT];  // this thread's of them
+    double t_mass = 0.0;
+    if (by_p && !by_k && r.weight.plain) {
+        // top-p alone: the counts of the distances say about where its
+        // threshold is.  One pass then takes exact sums, of everything and of
+        // what lies before that place, and lists the tokens around it.  Where
+        // the sums show it to be among those, the rest is work on the lists;
+        // else nothing is lost but the pass.  (Masses of all bins are four
+        // atomics per token: 64 x 128256 fp32 took 140 us, so 108.)
+        r.count_distances(true);
+        int b0, b1;
+        // (as wide as the lists bear where a share of the mass has up to
+        // sixteen times its share of the tokens)
+        r.mass_range(top_p, fminf(0.01f, (float)size * (kList / 16) / (float)a.vocab), b0, b1);
+        const float d0 = near_edge(b0), d1 = far_edge(b1);
+        u64 all = 0;
+        for (int j = v0; j < v1; ++j) {
+            float v[E];
+            Row<XT>::unpack(vec[j], v);
+#pragma unroll
+            for (int k = 0; k < E; k += 2) {
+                const auto w = r.weight.fast(v[k], v[k + 1]);
+                all += w.x + w.y;
+                own += (top - v[k] < d0 ? w.x : 0) + (top - v[k + 1] < d0 ? w.y : 0);
+            }
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                const float d = top - v[k];  // (neither -inf nor NaN passes d < d1)
+                if (d >= d0 && d < d1) {
+                    const uint32_t at = atomicAdd(&s.list_n, 1u);
+                    if (at < (uint32_t)kList) s.list[at] = order_key(v[k], (uint32_t)(r.lo + j * E + k));
+                }
+            }
+        }
+        u64 cta_all, cta_before;
+        r.block_before(all, cta_all);
+        r.block_before(own, cta_before);
+        const bool full = s.list_n > (uint32_t)kList;
+        if (threadIdx.x < size) {
+            st_cluster(mapa(&s.slot[0][rank], threadIdx.x), cta_all);
+            st_cluster(mapa(&s.slot[1][rank], threadIdx.x), cta_before | (full ? 1ull << 63 : 0));
+        }
+        csync();
+        u64 before = 0;
+        for (int q = 0; q < size; ++q) {
+            mass += s.slot[0][q];
+            before |= s.slot[1][q] & (1ull << 63);
+            before += s.slot[1][q] & ~(1ull << 63);
+        }
+        t_mass = (double)top_p * (double)mass;
+        if (!(before >> 63) && (double)before < t_mass) {
+            // a histogram of the listed ones, and the members of its bin
+            const uint32_t lo_bits = b0 ? __float_as_uint(d0) : 0, span = __float_as_uint(d1) - lo_bits;
+            int sh = 0;
+            while (((span - 1) >> sh) >= (uint32_t)kBins) ++sh;
+            const int m = (int)s.list_n;
+            r.clear_hist();
+            auto bin_of = [&](u64 key) {
+                return (int)((__float_as_uint(top - from_desc((uint32_t)(key >> 32))) - lo_bits) >> sh);
+            };
+#pragma unroll
+            for (int j = 0; j < kList / kT; ++j) {
+                const int i = threadIdx.x + j * kT;
+                mine[j] = i < m ? s.list[i] : kNoKey;
+                if (i < m) r.add(bin_of(mine[j]), from_desc((uint32_t)(mine[j] >> 32)), true);
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) s.list_n = 0;
+            r.merge_hist();
+            const auto p = r.pick_bin(true, 0, before, t_mass);
+            near = p.bin < kBins && p.in_cnt <= (uint32_t)kList;
+            if (near) {
+#pragma unroll
+                for (int j = 0; j < kList / kT; ++j)
+                    if (mine[j] != kNoKey && bin_of(mine[j]) == p.bin) s.list[atomicAdd(&s.list_n, 1u)] = mine[j];
+                mass = before + p.before_mass;
+            } else {
+                csync();  // (the histogram is about to be cleared)
+            }
+        }
+    }
+    // first by count, then by mass
+    bool l1 = false;
+    for (int by_mass = by_k ? 0 : 1; by_mass < (by_p ? 2 : 1); ++by_mass) {
+        if (by_mass && !by_k && !near) {  // the whole mass first: one histogram serves both
+            r.build_l1(true);
+            l1 = true;
+            mass = r.l1_mass();
+        }
+        if (!near) t_mass = (double)top_p * (double)mass;
+        thr = r.select(by_mass != 0, (uint32_t)top_k, t_mass, thr, by_p, near, l1, mass);
+    }
+
+    // the kept mass
     const float thr_v = thr == kNoKey ? -INFINITY : from_desc((uint32_t)(thr >> 32));
     const int thr_i = (int)(uint32_t)thr;
-    auto kept = [&](float v, int i) -> u64 {
-        if (!(v > thr_v) && (v != thr_v || i > thr_i)) return 0;  // behind the threshold
-        const u64 w = r.weight(v);
-        return w >= least_w ? w : 0;
+    auto kept = [&](float v, int i, u64 w) -> u64 {  // w, or 0 behind the threshold or below min-p
+        return (v > thr_v || (v == thr_v && i <= thr_i)) && w >= least_w ? w : 0;
     };
-    u64 own = 0;
-    if (!filtered) {
-        for (int j = v0; j < v1; ++j) {
-            float v[E];
-            Row<XT>::unpack(vec[j], v);
+    if (near && least_w == 0) {
+        // what lies before the listed ones is summed up already; of those, the
+        // ones up to the threshold go to their runs (in the merged masses' words)
+        s.mmass[threadIdx.x] = 0;
+        __syncthreads();
 #pragma unroll
-            for (int k = 0; k < E; ++k) own += r.weight.fast(v[k]);
-        }
+        for (int j = 0; j < kList / kT; ++j)
+            if (mine[j] != kNoKey && mine[j] <= thr)
+                atomicAdd(&s.mmass[((uint32_t)mine[j] - r.lo) / E / run], r.weight.fast(from_desc((uint32_t)(mine[j] >> 32))));
+        __syncthreads();
+        own += s.mmass[threadIdx.x];
+    } else if (own = 0; r.weight.plain) {
+        auto pairs = [&](auto f) {
+            for (int j = v0; j < v1; ++j) {
+                float v[E];
+                Row<XT>::unpack(vec[j], v);
+#pragma unroll
+                for (int k = 0; k < E; k += 2) own += f(v[k], v[k + 1], r.lo + j * E + k, r.weight.fast(v[k], v[k + 1]));
+            }
+        };
+        if (thr == kNoKey && least_w == 0) pairs([&](float, float, int, auto w) { return w.x + w.y; });
+        else pairs([&](float x, float y, int i, auto w) { return kept(x, i, w.x) + kept(y, i + 1, w.y); });
     } else {
-        for (int j = v0; j < v1; ++j) {
-            float v[E];
-            Row<XT>::unpack(vec[j], v);
-#pragma unroll
-            for (int k = 0; k < E; ++k) own += kept(v[k], r.lo + j * E + k);
+        for (int i = v0 * E; i < v1 * E; ++i) {
+            const float v = to_f32(reinterpret_cast<const XT*>(vec)[i]);
+            own += kept(v, r.lo + i, r.weight.general(v));
         }
     }
     u64 cta;
@@ -927,7 +1078,7 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const SampleArgs a) {
         for (int i0 = e0; i0 < e1; i0 += 32) {
             const int i = i0 + lane;
             const float v = i < e1 ? to_f32(reinterpret_cast<const XT*>(vec)[i]) : -INFINITY;
-            const u64 m = filtered ? kept(v, r.lo + i) : r.weight.fast(v);
+            const u64 m = kept(v, r.lo + i, r.weight(v));
             const u64 incl = before + warp_scan(m, lane);
             const uint32_t hit = __ballot_sync(0xffffffffu, (double)incl > t);
             if (hit) {

@@ -211,3 +211,38 @@ def test_writes_its_rows_only_and_refuses():
         cb.sample_tokens(torch.zeros(1, 327681, device=DEV), u[:1])
     assert e.value.code == cb.COTTUS_ERR_UNSUPPORTED
     assert cb.sample_tokens(x[:0], u[:0]).shape == (0,)
+
+
+@pytest.mark.parametrize("batch", [1, 64, 320])
+def test_top_p_alone(batch):
+    """Rows on which a count of the distances says much, little or something wrong about where the mass ends: smooth,
+    peaked, sorted (one part of the row holds every likely token), crowded just below the maximum, in a few steps, at
+    steep and flat temperatures, with shares of nearly nothing and nearly everything."""
+    vocab = 30011
+    g = torch.Generator().manual_seed(21)
+    rows = [torch.randn(vocab, generator=g) * s for s in (0.02, 1.0, 4.0)]
+    rows.append(torch.randn(vocab, generator=g).sort(descending=True).values * 2)
+    peaked = torch.randn(vocab, generator=g)
+    peaked[torch.randint(vocab, (30,), generator=g)] += 9 + torch.rand(30, generator=g)
+    rows.append(peaked)
+    crowded = torch.randn(vocab, generator=g) - 6
+    crowded[::20] = 4.0 + 0.02 * torch.rand(crowded[::20].numel(), generator=g)
+    crowded[77] = 4.25
+    rows += [crowded, (torch.randn(vocab, generator=g) * 2).round(), torch.linspace(-30, 5, vocab)]
+    n = len(rows)
+    shares, temps = (1e-6, 0.1, 0.5, 0.9, 0.99, 0.999999), (0.05, 0.7, 1.0, 30.0)
+    cases = [(i % n, float(np.float32(shares[(i // 3) % 6])), float(np.float32(temps[i % 4]))) for i in range(batch)]
+    logits = torch.stack([rows[r] for r, _, _ in cases])
+    u = torch.rand(batch, generator=g)
+    p, t = torch.tensor([c[1] for c in cases]), torch.tensor([c[2] for c in cases])
+    got = cb.sample_tokens(logits.to(DEV), u.to(DEV), temperature=t.to(DEV), top_p=p.to(DEV))
+    again = cb.sample_tokens(logits.to(DEV), u.to(DEV), temperature=t.to(DEV), top_p=p.to(DEV))
+    assert torch.equal(got, again)
+    known = 0
+    for b in range(0, batch, max(1, batch // 96)):
+        want, _, _ = ref.sample(logits[b].numpy(), float(u[b]), cases[b][2], 0, cases[b][1])
+        if want is None:
+            continue
+        known += 1
+        assert int(got[b]) == want, (b, cases[b])
+    assert known >= min(batch, 96) * 0.8
