@@ -23,6 +23,10 @@
 // TMEM holds two to four product buffers, so the tensor cores work on one
 // group while another is being added up.
 //
+// Up to 16 rows of x by a small weight go to fp8_linear_thin_kernel, which
+// takes the weight straight to registers: without barriers, tensor memory and
+// clusters to set up, one row by 2048 x 2048 takes 2.4 us against 4.5.
+//
 // Two tiles:
 //   narrow  128 rows of the weight (TMEM lanes) by XR = 16, 32, 64 or 128 rows
 //           of x (columns), one CTA.  A decode batch reads the weight once and
@@ -799,6 +803,114 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
     if (warp == kSumWarps + 1) tmem_free<PAIR>(tmem, tmem_cols);
 }
 
+// ---------------------------------------------------------------------------
+// few rows of x by a small weight
+// ---------------------------------------------------------------------------
+constexpr int kThinTile = 16;   // rows of the weight per CTA
+constexpr int kThinWarps = 16;  // each takes every 16th group
+
+// Two e4m3 values as two fp16 ones (exact).
+__device__ __forceinline__ uint32_t half2_of(uint32_t e4m3x2) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)e4m3x2));
+    return r;
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Up to 8 NT rows of x by 16 rows of the weight per CTA.  No shared memory,
+// tensor memory or cluster on the way of the weight: a lane loads 16 bytes each
+// of weight rows l / 4 and l / 4 + 8 and of rows l / 4 (+ 8 ...) of x at the same
+// columns, which is what it needs for four multiplies, as long as both sides
+// number the columns alike (in the multiply's terms columns 2t, 2t + 1, 2t + 8
+// and 2t + 9 of step i are bytes 4i to 4i + 3 of the lane's 16).  Products of
+// two e4m3 values are exact in fp16's tensor core and its sums fp32.
+template <int NT>
+__global__ void __launch_bounds__(kThinWarps * 32) fp8_linear_thin_kernel(const uint8_t* __restrict__ x,
+                                                                          const uint8_t* __restrict__ w, const LinArgs a,
+                                                                          const int K) {
+    __shared__ float part[kThinWarps][kThinTile][8 * NT + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+    const int n0 = blockIdx.x * kThinTile;
+    const bool live0 = n0 + r < a.N, live1 = n0 + r + 8 < a.N;
+    const uint8_t* w0 = w + (size_t)(n0 + r) * K + t * 16;
+    const uint8_t* w1 = w0 + (size_t)8 * K;
+    const uint8_t* xr = x + (size_t)r * K + t * 16;
+    const float* ws = a.ws + (size_t)(n0 / 128) * a.groups;
+    // (the first weights' way to L2 before the preceding kernel is done: a hint, as above)
+    if (t == 0 && live0 && warp * kBK < K) asm volatile("prefetch.global.L2 [%0];" ::"l"(w0 + warp * kBK));
+    if (t == 0 && live1 && warp * kBK < K) asm volatile("prefetch.global.L2 [%0];" ::"l"(w1 + warp * kBK));
+    grid_dependency_wait();
+    grid_dependents_launch();
+    float sum[NT][4] = {};
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (int g = warp; g < a.groups; g += kThinWarps) {
+        uint4 wa[2], wb[2], xv[2][NT];
+        float s[NT][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c = g * kBK + h * 64;
+            const bool in = c + t * 16 < K;
+            wa[h] = in && live0 ? ld_once(w0 + c) : zero;
+            wb[h] = in && live1 ? ld_once(w1 + c) : zero;
+#pragma unroll
+            for (int q = 0; q < NT; ++q)
+                xv[h][q] = in && r + q * 8 < a.M ? *reinterpret_cast<const uint4*>(xr + (size_t)q * 8 * K + c) : zero;
+        }
+        const float sw = ws[g];
+        const float* xs = a.xs + (size_t)g * a.M;
+#pragma unroll
+        for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int m = q * 8 + 2 * t + j;
+                s[q][j] = m < a.M ? xs[m] * sw : 0.f;
+            }
+        float d[NT][4] = {};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t ua[4] = {wa[h].x, wa[h].y, wa[h].z, wa[h].w}, ub[4] = {wb[h].x, wb[h].y, wb[h].z, wb[h].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t f[4] = {half2_of(ua[i]), half2_of(ub[i]), half2_of(ua[i] >> 16), half2_of(ub[i] >> 16)};
+#pragma unroll
+                for (int q = 0; q < NT; ++q) {
+                    const uint32_t ux = i == 0 ? xv[h][q].x : (i == 1 ? xv[h][q].y : (i == 2 ? xv[h][q].z : xv[h][q].w));
+                    mma_16816(d[q], f, half2_of(ux), half2_of(ux >> 16));
+                }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < NT; ++q)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[q][j] = fmaf(d[q][j], s[q][j & 1], sum[q][j]);
+    }
+#pragma unroll
+    for (int q = 0; q < NT; ++q)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) part[warp][r + (j >> 1) * 8][q * 8 + 2 * t + (j & 1)] = sum[q][j];
+    __syncthreads();
+    const int row = threadIdx.x & 15, n = n0 + row, m = threadIdx.x >> 4;
+    if (m < a.M && n < a.N) {
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < kThinWarps; ++q) v += part[q][row][m];
+        const size_t e = (size_t)m * a.N + n;
+        if (a.residual) v += a.residual[e];
+        if (a.out_dtype == COTTUS_F32) reinterpret_cast<float*>(a.out)[e] = v;
+        else if (a.out_dtype == COTTUS_F16) reinterpret_cast<__half*>(a.out)[e] = __float2half_rn(v);
+        else reinterpret_cast<__nv_bfloat16*>(a.out)[e] = __float2bfloat16_rn(v);
+    }
+}
+template <int NT>
+cudaError_t launch_thin(const cottus_fp8_linear_params* p, const LinArgs& a, cudaStream_t st) {
+    return launch_pdl(fp8_linear_thin_kernel<NT>, dim3((unsigned)((a.N + kThinTile - 1) / kThinTile)), dim3(kThinWarps * 32), 0,
+                      st, static_cast<const uint8_t*>(p->x), static_cast<const uint8_t*>(p->weight), a, p->in_features);
+}
+
 int fail(int code, const std::string& msg) { return set_error(code, msg); }
 
 // What a device allows, found at its first call.
@@ -952,11 +1064,22 @@ extern "C" int cottus_fp8_linear(const cottus_fp8_linear_params* p, cottus_strea
     const int64_t narrow = (int64_t)((M + 127) / 128) * ((N + 127) / 128), wide = (int64_t)((M + 255) / 256) * ((N + 255) / 256);
     if (narrow >= (int64_t(1) << 30)) return fail(COTTUS_ERR_UNSUPPORTED, "product too large");
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    // The wide tile where the narrow ones do not fit the GPU at once.  K = 4096,
-    // narrow against wide in us: 144 narrow tiles (384 x 6144) 15.4 : 19.4,
-    // 192 (512 x 6144) 25.2 : 19.6, 384 (1024 x 6144) 36.7 : 34.0, 1152 (3000 x
-    // 6144) 90 : 71.  Up to 128 rows half of the wide tile would be empty.
-    if (M > 128 && dev.pairs > 0 && narrow > dev.sms) {
+    // The thin kernel while its CTAs are few and short, against the narrow tile
+    // in us, one row: 1000 x 512 1.6 : 3.1, 2048 x 2048 2.4 : 4.5, 4096 x 4096 4.9 :
+    // 6.9, 6144 x 4096 7.8 : 8.9, 9472 x 512 3.9 : 4.1; 16384 x 1024 8.6 : 5.6, 32000 x
+    // 2048 17.9 : 14.8, 512 x 28672 18.6 : 11.1.  16 rows (its registers then
+    // leave one CTA per SM): 2368 x 4096 4.6 : 6.2, 2048 x 2048 2.8 : 4.6; 4096 x
+    // 4096 8.5 : 7.1, 1184 x 8192 7.5 : 6.4.
+    const int64_t thin = (N + kThinTile - 1) / kThinTile;
+    if (M <= 8 && thin <= 4 * dev.sms && groups <= 4 * kThinWarps) {
+        e = launch_thin<1>(p, a, st);
+    } else if (M <= 16 && thin <= dev.sms && groups <= 2 * kThinWarps) {
+        e = launch_thin<2>(p, a, st);
+    } else if (M > 128 && dev.pairs > 0 && narrow > dev.sms) {
+        // The wide tile where the narrow ones do not fit the GPU at once.  K = 4096,
+        // narrow against wide in us: 144 narrow tiles (384 x 6144) 15.4 : 19.4,
+        // 192 (512 x 6144) 25.2 : 19.6, 384 (1024 x 6144) 36.7 : 34.0, 1152 (3000 x
+        // 6144) 90 : 71.  Up to 128 rows half of the wide tile would be empty.
         a.m_tiles = (M + 255) / 256;
         a.n_tiles = (N + 255) / 256;
         a.splits = 1;

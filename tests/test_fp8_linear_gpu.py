@@ -88,7 +88,9 @@ def test_against_64_bits(m, n, k, out_dtype, residual):
 # the wide tile with rows that its stores cannot take whole
 BORDERS = [(m, n, k) for m in (2, 15, 17, 31, 32, 33, 63, 65, 96) for n, k in ((260, 1040), (20001, 2064))] + \
     [(16, 128 * t, 1152) for t in (1, 13, 18, 22, 29, 37, 49, 73, 74, 100, 148, 149)] + \
-    [(900, 3001, 400), (513, 9000, 16), (257, 10001, 128)]
+    [(17, 128 * t, 1152) for t in (1, 13, 18)] + [(900, 3001, 400), (513, 9000, 16), (257, 10001, 128)] + \
+    [(m, n, k) for m in (1, 7, 8, 9, 16) for n, k in ((16, 16), (17, 2048), (2368, 4096), (2369, 4112), (9472, 1040), (9489, 144),
+                                                     (130, 8192), (130, 8208))]
 
 
 @pytest.mark.parametrize("m, n, k", BORDERS)
