@@ -829,8 +829,7 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
 // and 2t + 9 of step i are bytes 4i to 4i + 3 of the lane's 16).  Products of
 // two e4m3 values are exact in fp16's tensor core and its sums fp32.
 template <int NT>
-__global__ void __launch_bounds__(kThinWarps * 32) fp8_linear_thin_kernel(const uint8_t* __restrict__ x,
-                                                                          const uint8_t* __restrict__ w, const LinArgs a,
+__global__ void __launch_bounds__(kThinWarps * 32) fp8_linear_thin_kernel(const uint8_t* x, const uint8_t* w, const LinArgs a,
                                                                           const int K) {
     __shared__ float part[kThinWarps][kThinTile][8 * NT + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
@@ -858,6 +857,7 @@ __global__ void __launch_bounds__(kThinWarps * 32) fp8_linear_thin_kernel(const 
             wb[h] = in && live1 ? ld_once(w1 + c) : zero;
 #pragma unroll
             for (int q = 0; q < NT; ++q)
+                // (no restricted pointers here: a read that counts as constant might move ahead of the wait)
                 xv[h][q] = in && r + q * 8 < a.M ? *reinterpret_cast<const uint4*>(xr + (size_t)q * 8 * K + c) : zero;
         }
         const float sw = ws[g];

@@ -186,18 +186,19 @@ def test_two_streams_at_once():
         assert torch.equal(tok, want[i][0]) and torch.equal(logits, want[i][1])
 
 
-def test_weights_written_just_before():
+@pytest.mark.parametrize("rows", [1, 5, 16, 70])
+def test_weights_written_just_before(rows):
     """A projection right behind the kernel that writes its weight, and behind the one that writes its input, over and
     over without waiting: it may prefetch, but not read, before they are done."""
     g = torch.Generator(device=DEV).manual_seed(6)
     ws = [torch.randn(1024, HIDDEN, generator=g, device=DEV) for _ in range(3)]
-    xs = [torch.randn(70, HIDDEN, generator=g, device=DEV) for _ in range(3)]
+    xs = [torch.randn(rows, HIDDEN, generator=g, device=DEV) for _ in range(3)]
     want = []
     for w, x in zip(ws, xs):
         want.append(cb.fp8_linear(*cb.quantize_fp8(x), *cb.quantize_fp8(w, block_rows=128), out_dtype=torch.float32))
         torch.cuda.synchronize()
     wq, wsc = torch.empty(1024, HIDDEN, dtype=FP8, device=DEV), torch.empty(8, HIDDEN // 128, device=DEV)
-    xq, xsc = torch.empty(70, HIDDEN, dtype=FP8, device=DEV), torch.empty(HIDDEN // 128, 70, device=DEV)
+    xq, xsc = torch.empty(rows, HIDDEN, dtype=FP8, device=DEV), torch.empty(HIDDEN // 128, rows, device=DEV)
     outs = []
     for i in range(60):
         cb.quantize_fp8(xs[i % 3], out=xq, scales=xsc)
