@@ -110,19 +110,18 @@ struct Vec8 {
             return amax8(v);
         } else {
             const uint32_t m = max2_abs(max2_abs(w[0], w[1]), max2_abs(w[2], w[3]));
-            return max_nan(to_f32(half_of(m)), to_f32(half_of(m >> 16)));
+            return max_nan(fabsf(to_f32(half_of(m))), fabsf(to_f32(half_of(m >> 16))));
         }
     }
     __device__ __forceinline__ static XT half_of(uint32_t x) {
         const uint16_t b = (uint16_t)x;
         return *reinterpret_cast<const XT*>(&b);
     }
+    // (with the product's sign)
     __device__ __forceinline__ static uint32_t max2_abs(uint32_t a, uint32_t b) {
-        a &= 0x7FFF7FFFu;
-        b &= 0x7FFF7FFFu;
         uint32_t r;
-        if constexpr (std::is_same<XT, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-        else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        if constexpr (std::is_same<XT, __half>::value) asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        else asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
         return r;
     }
     __device__ __forceinline__ void get(float (&v)[8]) const {

@@ -325,8 +325,8 @@ cudaError_t launch_quant(const QuantArgs& a, bool blocks, cudaStream_t st) {
         return launch_pdl(kern, dim3((unsigned)((a.rows + 16 * rt - 1) / (16 * rt) * tiles)), dim3(256), 0, st, a, (int)tiles);
     };
     // four groups per thread once the small tiles fill the GPU's 8 CTAs per SM:
-    // 16384 x 8192 fp16 84 us against 117, 64 x 4096 (128 small tiles) 2.2 against
-    // 1.5.  Element by element they do not help (8192 x 8191 bf16 117 against 79).
+    // 16384 x 8192 fp16 78 us against 97, 64 x 4096 (128 small tiles) 2.0 against
+    // 1.4.  Element by element they do not help (8192 x 8191 bf16 117 against 79).
     if constexpr (VEC) {
         int dev = 0;
         cudaGetDevice(&dev);
