@@ -302,3 +302,17 @@ print("same")
     out = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300,
                          env={**os.environ, "PYTHONPATH": str(root)})
     assert out.returncode == 0 and "same" in out.stdout, out.stderr[-2000:]
+
+
+def test_empty_batch():
+    """A step in which no sequence is active."""
+    layers, norm, head = _weights(9)
+    batch = cb.DecodeBatch(4, BS, 2, 2, device=DEV)
+    batch.begin_step()
+    tab = cb.rope_cos_sin_table(32, D).to(DEV)
+    pool = torch.zeros(4 * 2 * LAYERS * BS * HKV * D, dtype=torch.int16, device=DEV)
+    resid = torch.zeros(0, HIDDEN, device=DEV)
+    assert _block(batch, resid, layers[0], pool, tab, 0).shape == (0, H * D)
+    tokens, logits = cb.next_tokens(resid, norm, *head, torch.zeros(0, device=DEV))
+    assert tokens.shape == (0,) and logits.shape == (0, VOCAB)
+    torch.cuda.synchronize()
