@@ -166,11 +166,6 @@ struct Divisor {
     __device__ __forceinline__ explicit Divisor(float scale) : s(scale), r(0.f), plain(scale >= 0x1p-90f && scale < INFINITY) {
         if (plain) r = __frcp_rn(scale);
     }
-    __device__ __forceinline__ float quotient(float v) const {
-        if (!plain) return __fdiv_rn(v, s);
-        const float q0 = v * r;
-        return fmaf(fmaf(-q0, s, v), r, q0);
-    }
 };
 __device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], const Divisor& d) {
     float q[8];
@@ -194,9 +189,15 @@ __device__ __forceinline__ uint2 e4m3x8(const float (&v)[8], const Divisor& d) {
     o.y = e4m3x2(q[4], q[5]) | (e4m3x2(q[6], q[7]) << 16);
     return o;
 }
-// Eight values times the reciprocal of their group's scale: for values that
+// Four or eight values times the reciprocal of their group's scale: for values that
 // are rounded themselves, as a norm's are, where the quotient's last fp32 bit
 // is below their own error.
+__device__ __forceinline__ uint32_t e4m3x4_times(const float (&v)[4], const Divisor& d) {
+    float q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = d.plain ? v[j] * d.r : __fdiv_rn(v[j], d.s);
+    return e4m3x2(q[0], q[1]) | (e4m3x2(q[2], q[3]) << 16);
+}
 __device__ __forceinline__ uint2 e4m3x8_times(const float (&v)[8], const Divisor& d) {
     if (!d.plain) return e4m3x8(v, d);
     uint2 o;
@@ -204,7 +205,6 @@ __device__ __forceinline__ uint2 e4m3x8_times(const float (&v)[8], const Divisor
     o.y = e4m3x2(v[4] * d.r, v[5] * d.r) | (e4m3x2(v[6] * d.r, v[7] * d.r) << 16);
     return o;
 }
-__device__ __forceinline__ uint8_t e4m3(float v, const Divisor& d) { return (uint8_t)(e4m3x2(d.quotient(v), 0.f) & 0xFFu); }
 
 // ---------------------------------------------------------------------------
 // host

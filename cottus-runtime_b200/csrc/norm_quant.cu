@@ -128,6 +128,69 @@ __global__ void rms_norm_vec_kernel(const NormArgs a) {
     }
 }
 
+// Any width up to 16384 and any alignment: one CTA per row, G groups of 128 per
+// warp, the row in registers, four elements per lane and group (a warp reads 32
+// consecutive ones at a time).
+template <typename XT, int G>
+__global__ void __launch_bounds__(G == 1 ? 512 : 1024) rms_norm_elem_kernel(const NormArgs a) {
+    __shared__ float red[32];
+    const long long row = blockIdx.x;
+    const size_t base = (size_t)row * a.hidden;
+    const XT* x = reinterpret_cast<const XT*>(a.x) + base;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    grid_dependency_wait();
+    grid_dependents_launch();
+    // (element j of group g of this lane)
+    auto index = [&](int g, int j) { return (warp + g * warps) * 128 + j * 32 + lane; };
+    float h[G][4];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[g][j] = index(g, j) < a.hidden ? to_f32(x[index(g, j)]) : 0.f;
+    if (a.residual) {
+        const float* r = a.residual + base;
+        float* ro = a.residual_out + base;
+        float t[G][4];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[g][j] = index(g, j) < a.hidden ? r[index(g, j)] : 0.f;
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                h[g][j] += t[g][j];
+                if (index(g, j) < a.hidden) ro[index(g, j)] = h[g][j];
+            }
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ss = fmaf(h[g][j], h[g][j], ss);
+    ss = block_sum(ss, red);
+    const float inv = __frsqrt_rn(__fdiv_rn(ss, (float)a.hidden) + a.eps);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = index(g, j);
+            h[g][j] = i < a.hidden ? h[g][j] * inv * a.weight[i] : 0.f;
+            if (i < a.hidden && a.out_dtype != COTTUS_E4M3) store_out1(a.out, a.out_dtype, base + i, h[g][j]);
+            m = max_nan(m, fabsf(h[g][j]));
+        }
+        if (a.out_dtype != COTTUS_E4M3) continue;
+        m = amax16(m);
+        const float s = group_scale(max_nan(m, __shfl_xor_sync(0xffffffffu, m, 16)));
+        const uint32_t q = e4m3x4_times(h[g], Divisor(s));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (index(g, j) < a.hidden) reinterpret_cast<uint8_t*>(a.out)[base + index(g, j)] = (uint8_t)(q >> (8 * j));
+        if (lane == 0 && index(g, 0) < a.hidden) a.scales[(size_t)(warp + g * warps) * a.rows + row] = s;
+    }
+}
+
 // Any width and alignment: one CTA per row, the row read twice (the second
 // time from L1 or L2), one warp per group of 128.
 template <typename XT>
@@ -168,10 +231,11 @@ __global__ void __launch_bounds__(512) rms_norm_any_kernel(const NormArgs a) {
         }
         if (a.out_dtype == COTTUS_E4M3) {
             const float s = group_scale(max_nan(amax16(m), __shfl_xor_sync(0xffffffffu, amax16(m), 16)));
+            const uint32_t q = e4m3x4_times(y, Divisor(s));
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int i = g * 128 + j * 32 + lane;
-                if (i < a.hidden) reinterpret_cast<uint8_t*>(a.out)[base + i] = e4m3(y[j], Divisor(s));
+                if (i < a.hidden) reinterpret_cast<uint8_t*>(a.out)[base + i] = (uint8_t)(q >> (8 * j));
             }
             if (lane == 0) a.scales[(size_t)g * a.rows + row] = s;
         }
@@ -182,6 +246,13 @@ template <typename XT>
 cudaError_t launch_norm(const NormArgs& a, bool vec, cudaStream_t st) {
     // one row per CTA; the grid's x dimension holds any row count below 2^31
     if (!vec) {
+        // 8192 x 4095, fp32 with residual to fp16: 79 us against 132 with the row
+        // read twice; fp16 to e4m3 70 against 109; 64 x 8191 6.1 against 17.9
+        const int groups = (a.hidden + 127) / 128;
+        const dim3 rows((unsigned)a.rows);
+        if (groups <= 16) return launch_pdl(rms_norm_elem_kernel<XT, 1>, rows, dim3(groups * 32), 0, st, a);
+        if (groups <= 64) return launch_pdl(rms_norm_elem_kernel<XT, 2>, rows, dim3((groups + 1) / 2 * 32), 0, st, a);
+        if (groups <= 128) return launch_pdl(rms_norm_elem_kernel<XT, 4>, rows, dim3((groups + 3) / 4 * 32), 0, st, a);
         const int want = (a.hidden + 31) / 32 * 32;
         return launch_pdl(rms_norm_any_kernel<XT>, dim3((unsigned)a.rows), dim3(want < 512 ? want : 512), 0, st, a);
     }
@@ -248,9 +319,10 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const QuantArgs a, cons
         if constexpr (VEC) {
             if (lane * 8 < n) *reinterpret_cast<uint2*>(o + lane * 8) = e4m3x8(v, d);
         } else {
+            const uint2 q = e4m3x8(v, d);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (lane + j * 16 < n) o[lane + j * 16] = e4m3(v[j], d);
+                if (lane + j * 16 < n) o[lane + j * 16] = (uint8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
         }
         if (lane == 0) a.scales[(size_t)g * a.rows + row] = s;
     }
@@ -306,9 +378,10 @@ __global__ void __launch_bounds__(512, sizeof(XT) == 4 ? 2 : 3) quant_blocks_ker
         if constexpr (VEC) {
             if (lane * 8 < nc) *reinterpret_cast<uint2*>(o + lane * 8) = e4m3x8(v, d);
         } else {
+            const uint2 q = e4m3x8(v, d);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (lane + j * 16 < nc) o[lane + j * 16] = e4m3(v[j], d);
+                if (lane + j * 16 < nc) o[lane + j * 16] = (uint8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
         }
     }
     if (threadIdx.x == 0) a.scales[(size_t)rb * groups + cb] = s;

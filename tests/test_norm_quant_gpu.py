@@ -65,7 +65,8 @@ def _check_e4m3(y, q, s, rel):
 # one row to several waves; whole groups, ragged groups, odd widths, widths
 # around the register kernel's limits (8 * 512, 8 * 1024, 8 * 4096) and past them
 SHAPES = [(1, 2048), (3, 128), (5, 8), (2, 136), (7, 1), (4, 127), (3, 129), (6, 4096), (2, 4104), (2, 8192), (2, 8200),
-          (1, 32768), (1, 32776), (1000, 264), (33, 4999)]
+          (1, 32768), (1, 32776), (1000, 264), (33, 4999)] + \
+    [(70, 2047), (5, 2049), (4, 8191), (2, 8195), (3, 16383), (2, 16385), (1, 32767)]  # by groups of 128 per warp
 
 
 @pytest.mark.parametrize("rows, hidden", SHAPES)
