@@ -44,10 +44,22 @@ __device__ __forceinline__ uint4 ld_once(const void* p) {
                  : "l"(p));
     return r;
 }
+// (32-byte aligned: one access of 32 bytes per lane; two of 16, 32 bytes apart
+// from lane to lane, pass through L1 twice)
 __device__ __forceinline__ void load8_stream(const float* p, float (&v)[8]) {
-    const uint4 a = ld_once(p), b = ld_once(p + 4);
-    v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
-    v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
+    asm volatile("ld.global.L1::no_allocate.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "l"(p));
+}
+__device__ __forceinline__ void load8_kept(const float* p, float (&v)[8]) {
+    asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "l"(p));
+}
+__device__ __forceinline__ void store8_wide(float* p, const float (&v)[8]) {
+    asm volatile("st.global.v8.f32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+                 "f"(v[5]), "f"(v[6]), "f"(v[7]), "l"(p)
+                 : "memory");
 }
 __device__ __forceinline__ void load8_stream(const __half* p, float (&v)[8]) {
     const uint4 r = ld_once(p);

@@ -53,7 +53,7 @@ __device__ __forceinline__ float block_sum(float v, float* smem) {
 }
 
 __device__ __forceinline__ void store_out8(void* out, int dtype, size_t e, const float (&y)[8]) {
-    if (dtype == COTTUS_F32) store8(reinterpret_cast<float*>(out) + e, y);
+    if (dtype == COTTUS_F32) store8_wide(reinterpret_cast<float*>(out) + e, y);
     else if (dtype == COTTUS_F16) store8(reinterpret_cast<__half*>(out) + e, y);
     else store8(reinterpret_cast<__nv_bfloat16*>(out) + e, y);
 }
@@ -93,7 +93,7 @@ __global__ void rms_norm_vec_kernel(const NormArgs a) {
                 load8_stream(r + v * 8, t);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) h[i][j] += t[j];
-                store8(ro + v * 8, h[i]);
+                store8_wide(ro + v * 8, h[i]);
             }
         }
     }
@@ -109,7 +109,7 @@ __global__ void rms_norm_vec_kernel(const NormArgs a) {
         const int v = threadIdx.x + i * T;
         const bool live = v < nvec;
         float w[8];
-        if (live) load8(a.weight + v * 8, w);
+        if (live) load8_kept(a.weight + v * 8, w);
         else
 #pragma unroll
             for (int j = 0; j < 8; ++j) w[j] = 0.f;
@@ -456,8 +456,9 @@ int cottus_rms_norm(const cottus_rms_norm_params* p, cottus_stream_t stream) {
     a.out_dtype = p->out_dtype;
     a.eps = p->eps;
     // the register kernel holds rows of up to 32768 elements (4 vectors of 8 per thread)
-    const bool vec = p->hidden % 8 == 0 && p->hidden <= 32768 && aligned(p->x, 16) && aligned(p->residual, 16) &&
-                     aligned(p->residual_out, 16) && aligned(p->weight, 16) && aligned(p->out, os == 1 ? 8 : 16);
+    // and takes eight of them at a time
+    const bool vec = p->hidden % 8 == 0 && p->hidden <= 32768 && aligned(p->x, 8 * xs) && aligned(p->residual, 32) &&
+                     aligned(p->residual_out, 32) && aligned(p->weight, 32) && aligned(p->out, 8 * os);
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const cudaError_t e = p->x_dtype == COTTUS_F32   ? launch_norm<float>(a, vec, st)
                           : p->x_dtype == COTTUS_F16 ? launch_norm<__half>(a, vec, st)
