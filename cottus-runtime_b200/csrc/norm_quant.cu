@@ -52,6 +52,29 @@ __device__ __forceinline__ float block_sum(float v, float* smem) {
     return v;
 }
 
+// Sum over a row whose vector t + i T has the sum s[i] in thread t: by 32
+// neighbouring vectors, then over those, so that it does not depend on V and T
+// (a row comes out the same whatever the number of rows).
+template <int V>
+__device__ __forceinline__ float row_sum(float (&s)[V], float* smem, int nvec) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+        if (lane == 0) smem[i * warps + warp] = s[i];
+    }
+    __syncthreads();
+    const int blocks = (nvec + 31) >> 5;
+    float v = 0.f;  // (at most 1024 threads: 32 V such sums)
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (lane + i * 32 < blocks) v += smem[lane + i * 32];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
 __device__ __forceinline__ void store_out8(void* out, int dtype, size_t e, const float (&y)[8]) {
     if (dtype == COTTUS_F32) store8_wide(reinterpret_cast<float*>(out) + e, y);
     else if (dtype == COTTUS_F16) store8(reinterpret_cast<__half*>(out) + e, y);
@@ -67,7 +90,7 @@ __device__ __forceinline__ void store_out1(void* out, int dtype, size_t e, float
 // t, t + T, ... (V of them).  hidden a multiple of 8, all rows 16-byte aligned.
 template <typename XT, int V>
 __global__ void rms_norm_vec_kernel(const NormArgs a) {
-    __shared__ float red[32];
+    __shared__ float red[128];  // (one per 32 vectors of up to 4096)
     const int nvec = a.hidden >> 3, T = blockDim.x;
     const long long row = blockIdx.x;
     const XT* x = reinterpret_cast<const XT*>(a.x) + row * a.hidden;
@@ -97,12 +120,14 @@ __global__ void rms_norm_vec_kernel(const NormArgs a) {
             }
         }
     }
-    float ss = 0.f;
+    float part[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i)
+    for (int i = 0; i < V; ++i) {
+        part[i] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(h[i][j], h[i][j], ss);
-    ss = block_sum(ss, red);
+        for (int j = 0; j < 8; ++j) part[i] = fmaf(h[i][j], h[i][j], part[i]);
+    }
+    const float ss = row_sum<V>(part, red, nvec);
     const float inv = __frsqrt_rn(__fdiv_rn(ss, (float)a.hidden) + a.eps);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -259,8 +284,20 @@ cudaError_t launch_norm(const NormArgs& a, bool vec, cudaStream_t st) {
     const int nvec = a.hidden / 8;
     auto threads = [&](int V) { return ((nvec + V - 1) / V + 31) / 32 * 32; };
     const dim3 grid((unsigned)a.rows);
-    if (nvec <= 512) return launch_pdl(rms_norm_vec_kernel<XT, 1>, grid, dim3(threads(1)), 0, st, a);
-    if (nvec <= 1024) return launch_pdl(rms_norm_vec_kernel<XT, 2>, grid, dim3(threads(2)), 0, st, a);
+    // Vectors per thread.  One while every row has an SM to itself (100 x 4096
+    // fp16 + residual 2.7 us against 3.4 with two, 100 x 8192 fp32 2.3 : 2.5); beyond
+    // that two, so that several rows share an SM (16384 x 8192 bf16 + residual to
+    // e4m3 227 against 245 with one and 241 with four, 16384 x 4096 fp32 59 : 67 :
+    // 61); four where a row is 2 bytes per element and there are many (16384 x
+    // 8192 fp16 to e4m3 101 against 109 with two, 16384 x 2048 24 : 25; 600 x 8192 7.5 :
+    // 6.6), or where more than 768 threads would share a barrier (8192 x 16384 fp16
+    // + residual 248 : 292).
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const long long sms = device_sm_count(dev);
+    const bool thin = sizeof(XT) == 2 && !a.residual && a.rows > 8 * sms;
+    if (nvec <= 1024 && a.rows <= sms) return launch_pdl(rms_norm_vec_kernel<XT, 1>, grid, dim3(threads(1)), 0, st, a);
+    if (nvec <= 1536 && !thin) return launch_pdl(rms_norm_vec_kernel<XT, 2>, grid, dim3(threads(2)), 0, st, a);
     return launch_pdl(rms_norm_vec_kernel<XT, 4>, grid, dim3(threads(4)), 0, st, a);
 }
 

@@ -63,10 +63,11 @@ def _check_e4m3(y, q, s, rel):
 
 
 # one row to several waves; whole groups, ragged groups, odd widths, widths
-# around the register kernel's limits (8 * 512, 8 * 1024, 8 * 4096) and past them
+# around the register kernel's limits (8 * 1024, 8 * 2048, 8 * 4096) and past them
 SHAPES = [(1, 2048), (3, 128), (5, 8), (2, 136), (7, 1), (4, 127), (3, 129), (6, 4096), (2, 4104), (2, 8192), (2, 8200),
           (1, 32768), (1, 32776), (1000, 264), (33, 4999)] + \
-    [(70, 2047), (5, 2049), (4, 8191), (2, 8195), (3, 16383), (2, 16385), (1, 32767)]  # by groups of 128 per warp
+    [(70, 2047), (5, 2049), (4, 8191), (2, 8195), (3, 16383), (2, 16385), (1, 32767)] + \
+    [(149, 1032), (300, 8200), (150, 16384), (2, 16392), (1300, 136), (1200, 4104)]  # and by rows per SM
 
 
 @pytest.mark.parametrize("rows, hidden", SHAPES)
@@ -87,6 +88,23 @@ def test_rms_norm(rows, hidden, x_dtype, out_dtype, residual):
     else:
         assert got.dtype == out_dtype
         _check_y(y, got, rel)
+
+
+@pytest.mark.parametrize("hidden", [136, 1032, 4096, 8192, 8200, 12288, 16384, 32768])
+@pytest.mark.parametrize("x_dtype, residual", [(torch.float16, False), (torch.float32, True)])
+def test_rows_do_not_depend_on_their_number(hidden, x_dtype, residual):
+    """A row of a batch equals, bit for bit, the same row alone (the kernel's split of a row over threads differs)."""
+    x, w, r = (None if t is None else t.to(DEV) for t in _inputs(1300, hidden, x_dtype, residual))
+    for out_dtype in (torch.float32, FP8):
+        def norm(k):
+            got = cb.rms_norm(x[:k], w, residual=None if r is None else r[:k].clone(), out_dtype=out_dtype)
+            return (got[0].float(), got[1]) if out_dtype == FP8 else (got,)
+        full = norm(1300)
+        for k in (1, 140, 200):
+            part = norm(k)
+            assert torch.equal(part[0], full[0][:k])
+            if out_dtype == FP8:
+                assert torch.equal(part[1], full[1][:, :k])
 
 
 def test_rms_norm_buffers_and_aliases():
