@@ -304,6 +304,12 @@ def _operand(t: torch.Tensor, name: str, shape, dtypes, device: int) -> int:
     raise ValueError(f"{name} must be contiguous")
 
 
+def _device() -> int:
+    """The current device (torch.cuda.current_device without its check that CUDA is initialised, which a CUDA tensor
+    implies: 0.1 of its 0.2 us)."""
+    return torch._C._cuda_getDevice()
+
+
 def _raw_stream(stream, device: int):
     """The stream's handle; of the current stream without building a Stream object (3.4 us of a 13 us call)."""
     return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
@@ -339,13 +345,13 @@ def rms_norm(x, weight, *, eps=1e-5, residual=None, residual_out=None, out=None,
     torch.float8_e4m3fn, (y, scales): scales [ceil(hidden / 128)][rows] fp32, y = values * their group's scale."""
     if x.dim() != 2:
         raise ValueError("x must be [rows][hidden]")
-    dev = torch.cuda.current_device()
-    rows, hidden = x.shape
+    dev = _device()
+    shape = rows, hidden = x.shape
     p = RmsNormParams()
-    p.x = _operand(x, "x", x.shape, _DT_WIDE, dev)
+    p.x = _operand(x, "x", shape, _DT_WIDE, dev)
     p.weight = _operand(weight, "weight", (hidden,), _ONLY_F32, dev)
     if residual is not None:
-        p.residual = _operand(residual, "residual", x.shape, _ONLY_F32, dev)
+        p.residual = _operand(residual, "residual", shape, _ONLY_F32, dev)
         p.residual_out = p.residual if residual_out is None else _operand(residual_out, "residual_out", x.shape,
                                                                           _ONLY_F32, dev)
     elif residual_out is not None:
@@ -355,7 +361,7 @@ def rms_norm(x, weight, *, eps=1e-5, residual=None, residual_out=None, out=None,
     elif out_dtype is not None and out.dtype != out_dtype:
         raise TypeError(f"out is {out.dtype}, out_dtype is {out_dtype}")
     fp8 = out.dtype == _FP8
-    p.out = _operand(out, "out", x.shape, _ONLY_FP8 if fp8 else _DT_WIDE, dev)
+    p.out = _operand(out, "out", shape, _ONLY_FP8 if fp8 else _DT_WIDE, dev)
     if fp8:
         if scales is None:
             scales = _new(x, ((hidden + 127) // 128, rows), torch.float32, stream)
@@ -365,7 +371,7 @@ def rms_norm(x, weight, *, eps=1e-5, residual=None, residual_out=None, out=None,
     p.rows, p.hidden = rows, _i32(hidden, "hidden")
     p.x_dtype, p.out_dtype = _DT_WIDE[x.dtype], E4M3 if fp8 else _DT_WIDE[out.dtype]
     p.eps = eps
-    check(lib().cottus_rms_norm(C.byref(p), _raw_stream(stream, dev)))
+    check(lib().cottus_rms_norm(p, _raw_stream(stream, dev)))
     return (out, scales) if fp8 else out
 
 
@@ -375,7 +381,7 @@ def quantize_fp8(x, *, block_rows=1, out=None, scales=None, stream=None):
     block_rows 128: its weight, one scale per 128 x 128 block, [ceil(rows / 128)][ceil(cols / 128)]."""
     if x.dim() != 2:
         raise ValueError("x must be [rows][cols]")
-    dev = torch.cuda.current_device()
+    dev = _device()
     rows, cols = x.shape
     p = QuantizeParams()
     p.x = _operand(x, "x", x.shape, _DT_WIDE, dev)
@@ -388,7 +394,7 @@ def quantize_fp8(x, *, block_rows=1, out=None, scales=None, stream=None):
     p.out = _operand(out, "out", x.shape, _ONLY_FP8, dev)
     p.scales = _operand(scales, "scales", shape, _ONLY_F32, dev)
     p.rows, p.cols, p.x_dtype, p.block_rows = rows, _i32(cols, "cols"), _DT_WIDE[x.dtype], _i32(block_rows, "block_rows")
-    check(lib().cottus_quantize_fp8(C.byref(p), _raw_stream(stream, dev)))
+    check(lib().cottus_quantize_fp8(p, _raw_stream(stream, dev)))
     return out, scales
 
 
@@ -400,7 +406,7 @@ def fp8_linear(x, x_scales, weight, weight_scales, *, residual=None, out=None, o
     in a multiple of 16."""
     if x.dim() != 2 or weight.dim() != 2:
         raise ValueError("x must be [rows][in] and weight [out][in]")
-    dev = torch.cuda.current_device()
+    dev = _device()
     (rows, fin), fout = x.shape, weight.shape[0]
     groups = (fin + 127) // 128
     p = Fp8LinearParams()
@@ -417,7 +423,7 @@ def fp8_linear(x, x_scales, weight, weight_scales, *, residual=None, out=None, o
     p.out_dtype = _DT_WIDE[out.dtype]
     if status is not None:
         p.status = _operand(status, "status", (1,), _ONLY_I32, dev)
-    check(lib().cottus_fp8_linear(C.byref(p), _raw_stream(stream, dev)))
+    check(lib().cottus_fp8_linear(p, _raw_stream(stream, dev)))
     return out
 
 
@@ -430,7 +436,7 @@ def sample_tokens(logits, uniforms, *, temperature=None, top_k=None, top_p=None,
     without a finite logit), or (tokens, logprobs fp32 [batch]) with return_logprobs."""
     if logits.dim() != 2:
         raise ValueError("logits must be [batch][vocab]")
-    dev = torch.cuda.current_device()
+    dev = _device()
     batch, vocab = logits.shape
     row = (batch,)
     p = SampleParams()
@@ -454,7 +460,7 @@ def sample_tokens(logits, uniforms, *, temperature=None, top_k=None, top_p=None,
     if status is not None:
         p.status = _operand(status, "status", (1,), _ONLY_I32, dev)
     p.batch, p.vocab, p.dtype = _i32(batch, "batch"), _i32(vocab, "vocab"), _DT_WIDE[logits.dtype]
-    check(lib().cottus_sample_tokens(C.byref(p), _raw_stream(stream, dev)))
+    check(lib().cottus_sample_tokens(p, _raw_stream(stream, dev)))
     return (out, logprobs) if return_logprobs else out
 
 
