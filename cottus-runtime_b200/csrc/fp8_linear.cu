@@ -200,12 +200,6 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[32]) {
                        "+r"(v[i + 6]), "+r"(v[i + 7]));
 }
 
-// The box into L2 (a hint).
-__device__ __forceinline__ void tma_prefetch_l2(const CUtensorMap* map, int c0, int c1) {
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)),
-                 "r"(c0), "r"(c1)
-                 : "memory");
-}
 // 2-D tiled TMA store from this CTA's shared memory, in the thread's bulk group.
 __device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int c0, int c1) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
@@ -475,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_linear_kernel(const __grid_co
     // writes, L2 sees): 64 x 4096 x 4096 8.8 -> 8.6 us in a chain of launches
     if (warp == kSumWarps && first < tiles && elect_one()) {
         const int w0 = tile_n(first) + (PAIR ? rank * kWRows : 0);
-        for (int g = g0; g < g1 && g < g0 + kPrefetch; ++g) tma_prefetch_l2(&wmap, g * kBK, w0);
+        for (int g = g0; g < g1 && g < g0 + kPrefetch; ++g) tma_prefetch_l2_2d(&wmap, g * kBK, w0);
     }
     grid_dependency_wait();
     // (after the allocation above: a dependent that also allocates TMEM can

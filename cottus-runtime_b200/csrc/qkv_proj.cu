@@ -132,12 +132,13 @@ __global__ void __launch_bounds__(kQThreads) qkv_proj_kernel(const __grid_consta
         fence_barrier_init();
         failed = 0;
         issued = consumed = 0;
-        // the weights do not depend on the preceding kernel: the first stages'
-        // tiles are requested before waiting for it
-        for (int i = 0; i < npre; ++i) {
-            mbar_arrive_expect_tx(&full[i], STAGE);
-            tma_load_2d(smem + (size_t)i * STAGE, &wmap, &full[i], (split + i * a.splits) * kQK, row0);
-        }
+        // the first stages' weights start on their way to L2 before the
+        // preceding kernel is done; they are read after the wait, since that
+        // kernel may be the one that writes them (L2 sees what it still
+        // stores, shared memory would not).  Loaded before the wait, the
+        // O-projection took 11.9 us instead of 12.0, the QKV step 17.1
+        // instead of 17.3, and the attention block 122 as against 121.
+        for (int i = 0; i < npre; ++i) tma_prefetch_l2_2d(&wmap, (split + i * a.splits) * kQK, row0);
     }
     if (warp == 0) {  // accumulator: TMEM_COLS columns x 128 lanes
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
@@ -161,10 +162,8 @@ __global__ void __launch_bounds__(kQThreads) qkv_proj_kernel(const __grid_consta
             }
             uint8_t* st = smem + (size_t)slot * STAGE;
             const int kx = (split + i * a.splits) * kQK;
-            if (i >= npre) {
-                mbar_arrive_expect_tx(&full[slot], STAGE);
-                tma_load_2d(st, &wmap, &full[slot], kx, row0);
-            }
+            mbar_arrive_expect_tx(&full[slot], STAGE);
+            tma_load_2d(st, &wmap, &full[slot], kx, row0);
             tma_load_2d(st + W_BYTES, &xmap, &full[slot], kx, 0);
             issued = i + 1;
         }
@@ -214,8 +213,6 @@ __global__ void __launch_bounds__(kQThreads) qkv_proj_kernel(const __grid_consta
         // report, let the copies still in flight land (bounded), and go on
         // with zero partials
         report(a.status, COTTUS_STATUS_TIMEOUT);
-        // (the producer waits for nothing before it has requested the
-        // activations of the prefetched stages, so issued >= npre)
         for (int i = consumed; i < issued; ++i) (void)mbar_wait_bounded(&full[i % kQStages], (i / kQStages) & 1);
     }
     __syncthreads();
