@@ -1061,13 +1061,20 @@ extern "C" int cottus_fp8_linear(const cottus_fp8_linear_params* p, cottus_strea
     if (narrow >= (int64_t(1) << 30)) return fail(COTTUS_ERR_UNSUPPORTED, "product too large");
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     // The thin kernel while its CTAs are few and short, against the narrow tile
-    // in us, one row: 1000 x 512 1.6 : 3.1, 2048 x 2048 2.4 : 4.5, 4096 x 4096 4.9 :
-    // 6.9, 6144 x 4096 7.8 : 8.9, 9472 x 512 3.9 : 4.1; 16384 x 1024 8.6 : 5.6, 32000 x
-    // 2048 17.9 : 14.8, 512 x 28672 18.6 : 11.1.  16 rows (its registers then
-    // leave one CTA per SM): 2368 x 4096 4.6 : 6.2, 2048 x 2048 2.8 : 4.6; 4096 x
-    // 4096 8.5 : 7.1, 1184 x 8192 7.5 : 6.4.
+    // in us.  Up to 8 rows two CTAs share an SM.  All of them resident at once, one
+    // row: 1000 x 512 1.6 : 3.1, 2048 x 2048 2.4 : 4.5, 4096 x 4096 4.8 : 6.9, 4096 x
+    // 8192 8.2 : 10.1; 512 x 28672 18.6 : 11.1.  In two waves the second is part
+    // empty, which the narrow tile makes up for once a warp has more than two
+    // groups or the last of them leaves many warps idle: 6144 x 4096 7.7 : 8.9, 8192 x
+    // 4096 8.5 : 9.7, 9472 x 512 3.9 : 4.1, 6144 x 3584 7.9 : 8.2; 6144 x 2560 7.5 : 7.0,
+    // 5120 x 5120 9.8 : 8.8, 8192 x 8192 15.1 : 15.0, and with 8 rows 10.7 : 8.9 and
+    // 16.0 : 15.3.  Three waves: 16384 x 1024 8.6 : 5.6, 32000 x 2048 17.9 : 14.8.
+    // 16 rows (its registers then leave one CTA per SM): 2368 x 4096 4.6 : 6.2, 2048 x
+    // 2048 2.8 : 4.6; 4096 x 4096 8.5 : 7.1, 1184 x 8192 7.5 : 6.4.
     const int64_t thin = (N + kThinTile - 1) / kThinTile;
-    if (M <= 8 && thin <= 4 * dev.sms && groups <= 4 * kThinWarps) {
+    const int rounds = (groups + kThinWarps - 1) / kThinWarps;  // groups of a warp
+    const bool two_waves = thin <= 4 * dev.sms && (rounds == 1 || (rounds == 2 && groups >= 28));
+    if (M <= 8 && ((thin <= 2 * dev.sms && rounds <= 4) || two_waves)) {
         e = launch_thin<1>(p, a, st);
     } else if (M <= 16 && thin <= dev.sms && groups <= 2 * kThinWarps) {
         e = launch_thin<2>(p, a, st);
