@@ -50,13 +50,13 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <mutex>
 #include <string>
 
 #include "common.cuh"
 #include "cottus_b200.h"
 #include "internal.h"
 #include "lowp.cuh"
+#include "per_device.h"
 
 namespace cb200 {
 CUtensorMap make_tensor_map_2d_u8(const void* base, uint64_t inner, uint64_t outer, uint64_t pitch_bytes,
@@ -909,30 +909,13 @@ cudaError_t launch_thin(const cottus_fp8_linear_params* p, const LinArgs& a, cud
 
 int fail(int code, const std::string& msg) { return set_error(code, msg); }
 
-// What a device allows, found at its first call.
+// What a device allows, found at the first call that asks.
 struct DeviceLimits {
-    int sms = 0;
     int clusters[kMaxSplits + 1] = {};  // narrow-tile clusters of each size that are resident at once
-    int pairs = 0;                      // and wide-tile pairs (not every SM has a partner)
-    cudaError_t err = cudaSuccess;
+    int pairs = 0;                      // and wide-tile pairs (not every SM has a partner); 0: no wide tile
 };
-template <int XR, bool PAIR>
-cudaError_t set_up_kernel() {
-    auto kern = fp8_linear_kernel<XR, PAIR>;
-    cudaFuncAttributes fa = {};
-    cudaError_t e = cudaFuncGetAttributes(&fa, kern);
-    if (e != cudaSuccess) return e;
-    // (a warp is given registers in steps of 8 per thread)
-    if (PAIR && (fa.numRegs + 7) / 8 * 8 < kMinLaunchRegs) return cudaErrorInvalidConfiguration;
-    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
-}
-DeviceLimits find_limits(int dev) {
-    DeviceLimits l;
-    l.sms = device_sm_count(dev);
-    for (auto set_up : {set_up_kernel<16, false>, set_up_kernel<32, false>, set_up_kernel<64, false>,
-                        set_up_kernel<128, false>, set_up_kernel<128, true>})
-        if (l.err == cudaSuccess) l.err = set_up();
-    auto resident = [&](auto kern, int size, int* n) {
+cudaError_t find_limits(DeviceLimits& l) {
+    auto resident = [](auto kern, int size, int& n) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(size);
         cfg.blockDim = dim3(kThreads);
@@ -944,23 +927,28 @@ DeviceLimits find_limits(int dev) {
         attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        if (l.err == cudaSuccess) l.err = cudaOccupancyMaxActiveClusters(n, kern, &cfg);
+        return cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
     };
-    for (int s = 1; s <= kMaxSplits; ++s) resident(fp8_linear_kernel<128, false>, s, &l.clusters[s]);
-    resident(fp8_linear_kernel<128, true>, 2, &l.pairs);
-    return l;
+    cudaError_t e = cudaSuccess;
+    auto set_up = [&](auto kern) {
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
+    };
+    set_up(fp8_linear_kernel<16, false>);
+    set_up(fp8_linear_kernel<32, false>);
+    set_up(fp8_linear_kernel<64, false>);
+    set_up(fp8_linear_kernel<128, false>);
+    set_up(fp8_linear_kernel<128, true>);
+    for (int s = 1; s <= kMaxSplits && e == cudaSuccess; ++s) e = resident(fp8_linear_kernel<128, false>, s, l.clusters[s]);
+    // (a warp is given registers in steps of 8 per thread; compiled to fewer
+    // than its split needs, the wide tile is left out)
+    cudaFuncAttributes wide = {};
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&wide, fp8_linear_kernel<128, true>);
+    if (e == cudaSuccess && (wide.numRegs + 7) / 8 * 8 >= kMinLaunchRegs) e = resident(fp8_linear_kernel<128, true>, 2, l.pairs);
+    return e;
 }
-constexpr int kMaxDevices = 64;
-cudaError_t limits(DeviceLimits& l) {
-    static DeviceLimits cache[kMaxDevices];
-    static std::once_flag once[kMaxDevices];
-    int dev = 0;
-    const cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev >= kMaxDevices) return cudaErrorInvalidDevice;
-    std::call_once(once[dev], [&] { cache[dev] = find_limits(dev); });
-    l = cache[dev];
-    return l.err;
+cudaError_t limits(int dev, DeviceLimits& l) {
+    static PerDevice<DeviceLimits, cudaError_t> known;
+    return known.get(dev, l, cudaErrorInvalidDevice, find_limits);
 }
 
 template <int XR, bool PAIR>
@@ -1054,9 +1042,11 @@ extern "C" int cottus_fp8_linear(const cottus_fp8_linear_params* p, cottus_strea
     a.n_blocks = (N + 127) / 128;
     a.out_dtype = p->out_dtype;
     a.vec = N % 4 == 0 && aligned(p->out, es * 4) && aligned(p->residual, 16);
-    DeviceLimits dev;
-    cudaError_t e = limits(dev);
-    if (e != cudaSuccess) return fail(COTTUS_ERR_CUDA, std::string("CUDA error: ") + cudaGetErrorString(e));
+    auto cuda_fail = [](cudaError_t e) { return fail(COTTUS_ERR_CUDA, std::string("CUDA error: ") + cudaGetErrorString(e)); };
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return cuda_fail(e);
+    const int sms = device_sm_count(device);
     const int64_t narrow = (int64_t)((M + 127) / 128) * ((N + 127) / 128), wide = (int64_t)((M + 255) / 256) * ((N + 255) / 256);
     if (narrow >= (int64_t(1) << 30)) return fail(COTTUS_ERR_UNSUPPORTED, "product too large");
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -1073,12 +1063,19 @@ extern "C" int cottus_fp8_linear(const cottus_fp8_linear_params* p, cottus_strea
     // 2048 2.8 : 4.6; 4096 x 4096 8.5 : 7.1, 1184 x 8192 7.5 : 6.4.
     const int64_t thin = (N + kThinTile - 1) / kThinTile;
     const int rounds = (groups + kThinWarps - 1) / kThinWarps;  // groups of a warp
-    const bool two_waves = thin <= 4 * dev.sms && (rounds == 1 || (rounds == 2 && groups >= 28));
-    if (M <= 8 && ((thin <= 2 * dev.sms && rounds <= 4) || two_waves)) {
+    const bool two_waves = thin <= 4 * sms && (rounds == 1 || (rounds == 2 && groups >= 28));
+    if (M <= 8 && ((thin <= 2 * sms && rounds <= 4) || two_waves)) {
         e = launch_thin<1>(p, a, st);
-    } else if (M <= 16 && thin <= dev.sms && groups <= 2 * kThinWarps) {
+        return e == cudaSuccess ? COTTUS_OK : cuda_fail(e);
+    }
+    if (M <= 16 && thin <= sms && groups <= 2 * kThinWarps) {
         e = launch_thin<2>(p, a, st);
-    } else if (M > 128 && dev.pairs > 0 && narrow > dev.sms) {
+        return e == cudaSuccess ? COTTUS_OK : cuda_fail(e);
+    }
+    DeviceLimits dev;
+    e = limits(device, dev);
+    if (e != cudaSuccess) return cuda_fail(e);
+    if (M > 128 && dev.pairs > 0 && narrow > sms) {
         // The wide tile where the narrow ones do not fit the GPU at once.  K = 4096,
         // narrow against wide in us: 144 narrow tiles (384 x 6144) 15.4 : 19.4,
         // 192 (512 x 6144) 25.2 : 19.6, 384 (1024 x 6144) 36.7 : 34.0, 1152 (3000 x
@@ -1094,11 +1091,11 @@ extern "C" int cottus_fp8_linear(const cottus_fp8_linear_params* p, cottus_strea
         a.splits = 1;
         for (int s = 2; s <= kMaxSplits && s <= groups; ++s)
             if (narrow <= dev.clusters[s]) a.splits = s;
-        const int grid = a.splits > 1 ? (int)narrow * a.splits : (int)(narrow < dev.sms ? narrow : dev.sms);
+        const int grid = a.splits > 1 ? (int)narrow * a.splits : (int)(narrow < sms ? narrow : sms);
         e = M <= 16   ? launch_linear<16, false>(p, a, grid, st)
             : M <= 32 ? launch_linear<32, false>(p, a, grid, st)
             : M <= 64 ? launch_linear<64, false>(p, a, grid, st)
                       : launch_linear<128, false>(p, a, grid, st);
     }
-    return e == cudaSuccess ? COTTUS_OK : fail(COTTUS_ERR_CUDA, std::string("CUDA error: ") + cudaGetErrorString(e));
+    return e == cudaSuccess ? COTTUS_OK : cuda_fail(e);
 }
