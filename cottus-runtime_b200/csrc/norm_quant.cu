@@ -86,10 +86,15 @@ __device__ __forceinline__ void store_out1(void* out, int dtype, size_t e, float
     else reinterpret_cast<__nv_bfloat16*>(out)[e] = __float2bfloat16_rn(y);
 }
 
+// Threads per CTA at most (with 1024 a thread has up to 64 registers).
+template <int V>
+constexpr int kNormThreads = V == 2 ? 768 : 1024;
+
 // One CTA per row, the row in registers: thread t holds the vectors of eight
-// t, t + T, ... (V of them).  hidden a multiple of 8, all rows 16-byte aligned.
+// t, t + T, ... (V of them).  hidden a multiple of 8, rows 32-byte aligned in
+// fp32 and 16-byte aligned in 16 bits.
 template <typename XT, int V>
-__global__ void rms_norm_vec_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kNormThreads<V>) rms_norm_vec_kernel(const NormArgs a) {
     __shared__ float red[128];  // (one per 32 vectors of up to 4096)
     const int nvec = a.hidden >> 3, T = blockDim.x;
     const long long row = blockIdx.x;
@@ -296,8 +301,8 @@ cudaError_t launch_norm(const NormArgs& a, bool vec, cudaStream_t st) {
     cudaGetDevice(&dev);
     const long long sms = device_sm_count(dev);
     const bool thin = sizeof(XT) == 2 && !a.residual && a.rows > 8 * sms;
-    if (nvec <= 1024 && a.rows <= sms) return launch_pdl(rms_norm_vec_kernel<XT, 1>, grid, dim3(threads(1)), 0, st, a);
-    if (nvec <= 1536 && !thin) return launch_pdl(rms_norm_vec_kernel<XT, 2>, grid, dim3(threads(2)), 0, st, a);
+    if (nvec <= kNormThreads<1> && a.rows <= sms) return launch_pdl(rms_norm_vec_kernel<XT, 1>, grid, dim3(threads(1)), 0, st, a);
+    if (nvec <= 2 * kNormThreads<2> && !thin) return launch_pdl(rms_norm_vec_kernel<XT, 2>, grid, dim3(threads(2)), 0, st, a);
     return launch_pdl(rms_norm_vec_kernel<XT, 4>, grid, dim3(threads(4)), 0, st, a);
 }
 
