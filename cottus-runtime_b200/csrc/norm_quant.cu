@@ -289,14 +289,14 @@ cudaError_t launch_norm(const NormArgs& a, bool vec, cudaStream_t st) {
     const int nvec = a.hidden / 8;
     auto threads = [&](int V) { return ((nvec + V - 1) / V + 31) / 32 * 32; };
     const dim3 grid((unsigned)a.rows);
-    // Vectors per thread.  One while every row has an SM to itself (100 x 4096
-    // fp16 + residual 2.7 us against 3.4 with two, 100 x 8192 fp32 2.3 : 2.5); beyond
-    // that two, so that several rows share an SM (16384 x 8192 bf16 + residual to
-    // e4m3 227 against 245 with one and 241 with four, 16384 x 4096 fp32 59 : 67 :
-    // 61); four where a row is 2 bytes per element and there are many (16384 x
-    // 8192 fp16 to e4m3 101 against 109 with two, 16384 x 2048 24 : 25; 600 x 8192 7.5 :
-    // 6.6), or where more than 768 threads would share a barrier (8192 x 16384 fp16
-    // + residual 248 : 292).
+    // Vectors per thread (us, inputs in HBM).  One while every row has an SM to
+    // itself (100 x 4096 fp16 + residual 3.1 against 3.9 with two, 100 x 8192 fp32
+    // 3.4 : 3.5); beyond that two, so that several rows share an SM (16384 x 8192 bf16
+    // + residual to e4m3 228 against 243 with one and 240 with four, 16384 x 4096 fp32
+    // 80 : 82 : 81); four where a row is 2 bytes per element and there are many
+    // (16384 x 8192 fp16 to e4m3 104 against 114 with two, 16384 x 2048 27.6 : 28.3;
+    // 600 x 8192 7.9 : 7.1), or where more than 768 threads would share a barrier
+    // (8192 x 16384 fp16 + residual 248 : 282).
     int dev = 0;
     cudaGetDevice(&dev);
     const long long sms = device_sm_count(dev);
