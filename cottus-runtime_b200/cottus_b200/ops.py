@@ -6,6 +6,7 @@ tensors on the current device (the block pool helpers are host-only).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
@@ -46,21 +47,51 @@ def _require(t: torch.Tensor, name: str, dtype=None):
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
 
 
+def _on(stream):
+    """The context in which the caching allocator serves `stream` (None: the current one)."""
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
+def _capturing(device: torch.device) -> bool:
+    """Whether what the current stream does goes into a graph."""
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
+class _Scratch:
+    """Scratch memory that grows with what calls need.  Every buffer stays: a captured graph, or a kernel still running on
+    another stream, may hold an earlier, smaller one (each is at least twice the one before, so that they add up to
+    little).  A buffer made while a graph is captured is that graph's own, and with `cleared` cleared at each replay: until
+    the first replay nothing has written it, so no other call may have it."""
+
+    def __init__(self, device: torch.device, cleared: bool):
+        self.device, self.make, self.buffers = device, torch.zeros if cleared else torch.empty, []
+
+    def get(self, nbytes: int, stream=None) -> torch.Tensor:
+        """At least nbytes, allocated (and cleared) on the stream that uses them."""
+        last = self.buffers[-1].numel() if self.buffers else 1 << 19
+        if self.buffers and last >= nbytes:
+            return self.buffers[-1]
+        with _on(stream):
+            capturing = _capturing(self.device)
+            buf = self.make(max(nbytes, 0 if capturing else 2 * last), dtype=torch.uint8, device=self.device)
+        if not capturing:
+            self.buffers.append(buf)
+        return buf
+
+
 _WS: dict = {}
 
 
-def workspace(nbytes: int, device: torch.device, kind: str = "decode") -> torch.Tensor:
+def workspace(nbytes: int, device: torch.device, kind: str = "decode", stream=None) -> torch.Tensor:
     """Cached scratch buffer (a convenience of this Python layer; the C ABI
     itself only takes caller-provided workspace).  One buffer per kind: the
     decode kernels keep the counter words at the start of theirs at zero
     between calls, while the projections ("proj") overwrite all of theirs
     with split partials, so the two never share one."""
     key = (device.type, device.index, kind)
-    buf = _WS.get(key)
-    if buf is None or buf.numel() < nbytes:
-        buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        _WS[key] = buf
-    return buf
+    if key not in _WS:
+        _WS[key] = _Scratch(device, cleared=kind == "decode")
+    return _WS[key].get(nbytes, stream)
 
 
 def make_decode_params(out, query, kv_pool, block_table, context_lens, *, num_kv_heads, head_dim, block_size,
@@ -103,7 +134,7 @@ def paged_decode(query: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.
                            num_physical_blocks=num_physical_blocks, scale=scale, lse_out=lse_out, status=status)
     need = lib().cottus_paged_decode_workspace_size(C.byref(p))
     if need:
-        ws = workspace(need, query.device)
+        ws = workspace(need, query.device, stream=stream)
         p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
     check(lib().cottus_paged_decode(C.byref(p), _stream(stream)))
     return out
@@ -201,7 +232,7 @@ def rope_append_decode(query, key, value, positions, cos_sin, kv_pool, block_tab
                          query_out=query_out, out=out, scale=scale, status=status)
     need = lib().cottus_rope_append_decode_workspace_size(C.byref(p))
     if need:
-        ws = workspace(need, query.device) if workspace_of is None else workspace_of.workspace(need)
+        ws = workspace(need, query.device, stream=stream) if workspace_of is None else workspace_of.workspace(need, stream)
         p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
     check(lib().cottus_rope_append_decode(C.byref(p), _stream(stream)))
     return out
@@ -230,7 +261,7 @@ def qkv_rope_append(x, weight, positions, cos_sin, kv_pool, block_table, *, num_
     p.status = status.data_ptr() if status is not None else None
     need = lib().cottus_qkv_rope_append_workspace_size(C.byref(p))
     if need:
-        ws = workspace(need, x.device, "proj")
+        ws = workspace(need, x.device, "proj", stream)
         p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
     check(lib().cottus_qkv_rope_append(C.byref(p), _stream(stream)))
     return query_out
@@ -252,7 +283,7 @@ def o_proj_residual(x, weight, residual, *, out=None, out_dtype=torch.float32, s
     p.status = status.data_ptr() if status is not None else None
     need = lib().cottus_o_proj_residual_workspace_size(C.byref(p))
     if need:
-        ws = workspace(need, x.device, "proj")
+        ws = workspace(need, x.device, "proj", stream)
         p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
     check(lib().cottus_o_proj_residual(C.byref(p), _stream(stream)))
     return out
@@ -584,17 +615,16 @@ class DecodeBatch:
         self._h = h
         self.num_blocks, self.block_size = num_blocks, block_size
         self.max_batch, self.max_blocks_per_seq = max_batch, max_blocks_per_seq
-        self._workspaces = []  # (all of them: a captured graph may hold an earlier, smaller one)
+        if device is not None:
+            self._scratch = _Scratch(self.positions.device, cleared=True)
+            # before any capture, and for all grouped-query shapes enough (2.5 MB for 8 query heads of 128 per kv head)
+            self._scratch.get(4 << 20)
+            if self.positions.is_cuda and not _capturing(self.positions.device):
+                torch.cuda.current_stream(self.positions.device).synchronize()  # (the batch may be used on any stream)
 
-    def workspace(self, nbytes: int) -> torch.Tensor:
-        """This batch's scratch buffer for the decode kernels (whose counter words are zero between calls).  While a
-        graph is captured a buffer that does not exist yet is the graph's own, cleared at each replay."""
-        if self._workspaces and self._workspaces[-1].numel() >= nbytes:
-            return self._workspaces[-1]
-        buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=self.positions.device)
-        if not torch.cuda.is_current_stream_capturing():
-            self._workspaces.append(buf)
-        return buf
+    def workspace(self, nbytes: int, stream=None) -> torch.Tensor:
+        """This batch's scratch buffer for the decode kernels (whose counter words are zero between calls)."""
+        return self._scratch.get(nbytes, stream)
 
     def add(self, seq_id: int) -> int:
         row = C.c_int32()

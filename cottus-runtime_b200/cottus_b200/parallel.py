@@ -148,7 +148,7 @@ def split_kv_decode_peer(query, kv_pool, block_table, context_lens, exchange: Pe
                            num_physical_blocks=num_physical_blocks, lse_out=lse_out, status=status)
     need = lib().cottus_split_decode_workspace_size(C.byref(p))
     if need:
-        ws = workspace(need, query.device)
+        ws = workspace(need, query.device, stream=stream)
         p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
     check(lib().cottus_split_decode(C.byref(p), exchange._h, _stream(stream)))
     return out
