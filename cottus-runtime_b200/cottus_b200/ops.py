@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 
 import torch
 
@@ -50,6 +51,23 @@ def _require(t: torch.Tensor, name: str, dtype=None):
 def _on(stream):
     """The context in which the caching allocator serves `stream` (None: the current one)."""
     return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
+def _streamed(call):
+    """A call with a `stream` argument makes everything on that stream: what it allocates comes from that stream's memory
+    (of another's it might hold what that one still reads), and what it clears is cleared before it is written."""
+
+    @functools.wraps(call)
+    def on_its_stream(*args, stream=None, **kw):
+        if stream is None:
+            return call(*args, **kw)
+        if stream.device_index != torch.cuda.current_device():
+            raise ValueError(f"the stream is on cuda:{stream.device_index}, the current device is "
+                             f"cuda:{torch.cuda.current_device()}")
+        with _on(stream):
+            return call(*args, stream=stream, **kw)
+
+    return on_its_stream
 
 
 def _capturing(device: torch.device) -> bool:
@@ -117,6 +135,7 @@ def make_decode_params(out, query, kv_pool, block_table, context_lens, *, num_kv
     return p
 
 
+@_streamed
 def paged_decode(query: torch.Tensor, kv_pool: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor,
                  *, num_kv_heads: int, head_dim: int, block_size: int, num_layers: int = 1, layer: int = 0,
                  out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None, scale: float = 0.0,
@@ -144,6 +163,7 @@ def decode_workspace_size(p: PagedDecodeParams) -> int:
     return int(lib().cottus_paged_decode_workspace_size(C.byref(p)))
 
 
+@_streamed
 def lse_combine(partial_out: torch.Tensor, partial_lse: torch.Tensor, *, out: torch.Tensor | None = None,
                 out_dtype: torch.dtype = torch.float32, lse_out: torch.Tensor | None = None, stream=None):
     """Merge [P][B][H][D] normalised partials with their [P][B][H] LSEs."""
@@ -167,6 +187,7 @@ def rope_cos_sin_table(max_position: int, head_dim: int, theta: float = 10000.0)
     return t
 
 
+@_streamed
 def rope(x: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, *, out: torch.Tensor | None = None,
          stream=None) -> torch.Tensor:
     """RoPE of fp32 x[num_tokens][num_heads][head_dim] (in place when out is x)."""
@@ -206,6 +227,7 @@ def make_step_params(query, key, value, positions, cos_sin, kv_pool, block_table
     return p
 
 
+@_streamed
 def rope_append(query, key, value, positions, cos_sin, kv_pool, block_table, *, num_kv_heads, head_dim, block_size,
                 num_layers=1, layer=0, query_out=None, status=None, stream=None):
     """RoPE on the new token's q/k and KV append (cottus_rope_append)."""
@@ -218,6 +240,7 @@ def rope_append(query, key, value, positions, cos_sin, kv_pool, block_table, *, 
     return query_out
 
 
+@_streamed
 def rope_append_decode(query, key, value, positions, cos_sin, kv_pool, block_table, *, num_kv_heads, head_dim,
                        block_size, num_layers=1, layer=0, out=None, out_dtype=None, query_out=None, scale=0.0,
                        status=None, stream=None, workspace_of=None):
@@ -238,6 +261,7 @@ def rope_append_decode(query, key, value, positions, cos_sin, kv_pool, block_tab
     return out
 
 
+@_streamed
 def qkv_rope_append(x, weight, positions, cos_sin, kv_pool, block_table, *, num_heads, num_kv_heads, head_dim,
                     block_size, num_layers=1, layer=0, num_physical_blocks=None, query_out=None,
                     query_out_dtype=torch.float16, qkv_out=None, status=None, stream=None):
@@ -267,6 +291,7 @@ def qkv_rope_append(x, weight, positions, cos_sin, kv_pool, block_table, *, num_
     return query_out
 
 
+@_streamed
 def o_proj_residual(x, weight, residual, *, out=None, out_dtype=torch.float32, status=None, stream=None):
     """Output projection + residual add (cottus_o_proj_residual):
     out = x . weight^T + residual.  x [B][in] fp16, weight [out][in] fp16,
@@ -289,6 +314,7 @@ def o_proj_residual(x, weight, residual, *, out=None, out_dtype=torch.float32, s
     return out
 
 
+@_streamed
 def attention_block(batch, x, w_qkv, w_o, residual, kv_pool, cos_sin, *, num_heads, num_kv_heads, head_dim,
                     num_layers=1, layer=0, query_out=None, att_out=None, status=None, stream=None):
     """The attention half of one decoder layer for the step tokens of a
@@ -543,6 +569,7 @@ def next_tokens(residual, norm_weight, w_head, head_scales, uniforms, *, eps=1e-
     return tokens, logits
 
 
+@_streamed
 def paged_gather(kv_pool, block_table, context_lens, *, max_context, num_kv_heads, head_dim, block_size,
                  num_layers=1, layer=0, num_physical_blocks=None, status=None, k_out=None, v_out=None, stream=None):
     """Dense copy of the K and V rows named by the block table (bit-exact)."""

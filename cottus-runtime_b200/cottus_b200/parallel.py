@@ -19,7 +19,7 @@ import torch
 import torch.distributed as dist
 
 from ._lib import check, lib
-from .ops import _stream, lse_combine, make_decode_params, paged_decode, workspace
+from .ops import _stream, _streamed, lse_combine, make_decode_params, paged_decode, workspace
 
 
 def all_gather_partials(out: torch.Tensor, lse: torch.Tensor, group=None):
@@ -52,6 +52,7 @@ def gather_head_outputs(out: torch.Tensor, group=None) -> torch.Tensor:
     return torch.cat(parts, dim=1)
 
 
+@_streamed
 def split_kv_decode(query, kv_pool, block_table, context_lens, *, num_kv_heads, head_dim, block_size,
                     num_layers=1, layer=0, num_physical_blocks=None, out_dtype=torch.float16, group=None,
                     part=None, lse=None, stream=None):
@@ -133,6 +134,7 @@ class PeerExchange:
             self._h = None
 
 
+@_streamed
 def split_kv_decode_peer(query, kv_pool, block_table, context_lens, exchange: PeerExchange, *, num_kv_heads,
                          head_dim, block_size, num_layers=1, layer=0, num_physical_blocks=None,
                          out_dtype=torch.float16, out=None, lse_out=None, status=None, stream=None):

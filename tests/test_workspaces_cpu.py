@@ -92,6 +92,9 @@ def test_fused_calls_take_the_workspace_on_their_stream(capture, monkeypatch):
             seen.append(stream)
             raise KeyboardInterrupt  # (nothing is launched)
 
+    class Stream:
+        device_index = 0
+
     class Lib:
         @staticmethod
         def cottus_rope_append_decode_workspace_size(p):
@@ -100,8 +103,81 @@ def test_fused_calls_take_the_workspace_on_their_stream(capture, monkeypatch):
     monkeypatch.setattr(ops, "lib", lambda: Lib)
     monkeypatch.setattr(ops, "_require", lambda *a, **k: None)
     monkeypatch.setattr(ops, "make_step_params", lambda *a, **k: ops.DecodeStepParams())
-    x = torch.zeros(1, 2, 64)
+    monkeypatch.setattr(torch.cuda, "stream", lambda stream: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    x, side = torch.zeros(1, 2, 64), Stream()
     with pytest.raises(KeyboardInterrupt):
-        ops.rope_append_decode(x, x, x, x, x, x, x, num_kv_heads=2, head_dim=64, block_size=16, stream="side",
+        ops.rope_append_decode(x, x, x, x, x, x, x, num_kv_heads=2, head_dim=64, block_size=16, stream=side,
                                workspace_of=Batch())
-    assert seen == ["side"]
+    assert seen == [side]
+
+
+CALLS = [("paged_decode", 4), ("lse_combine", 2), ("rope", 3), ("rope_append", 7), ("rope_append_decode", 7),
+         ("qkv_rope_append", 6), ("o_proj_residual", 3), ("attention_block", 7), ("paged_gather", 3)]
+
+
+@pytest.mark.parametrize("name, args", CALLS)
+def test_a_stream_of_another_device_is_refused(monkeypatch, name, args):
+    """Its kernels would run on that device with this one's addresses."""
+
+    class Stream:
+        device_index = 1
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(ValueError, match="cuda:1.*cuda:0"):
+        getattr(cb, name)(*[torch.zeros(1, 2, 64)] * args, stream=Stream())
+
+
+@pytest.mark.parametrize("name, args", CALLS)
+def test_calls_run_within_their_stream(monkeypatch, name, args):
+    """Allocations of a call with a stream are served from that stream's memory."""
+    inside, log = [], []
+
+    class Stream:
+        device_index = 0
+
+    @contextlib.contextmanager
+    def on(stream):
+        inside.append(stream)
+        yield
+        inside.pop()
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "stream", on)
+
+    def stop(*a, **k):
+        log.append(list(inside))
+        raise KeyboardInterrupt
+
+    monkeypatch.setattr(ops, "_require", stop)
+    monkeypatch.setattr(ops, "qkv_rope_append", stop)
+    monkeypatch.setattr(torch, "zeros", stop)
+    side, x = Stream(), torch.ones(1, 2, 64)
+
+    class Batch:
+        num_blocks = 1
+
+        def __len__(self):
+            return 1
+
+        positions = block_table = context_lens = x
+
+        block_size = 16
+
+    kw = dict(num_kv_heads=2, head_dim=64, block_size=16)
+    if name == "attention_block":
+        kw = dict(num_heads=2, num_kv_heads=2, head_dim=64)
+    elif name == "qkv_rope_append":
+        monkeypatch.undo()
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+        monkeypatch.setattr(torch.cuda, "stream", on)
+        monkeypatch.setattr(ops, "_require", stop)
+        kw["num_heads"] = 2
+    elif name == "paged_gather":
+        kw["max_context"] = 16
+    elif name in ("lse_combine", "rope", "o_proj_residual"):
+        kw = {}
+    first = [Batch()] if name == "attention_block" else []
+    with pytest.raises(KeyboardInterrupt):
+        getattr(cb, name)(*first, *[x] * (args - len(first)), stream=side, **kw)
+    assert log == [[side]]
