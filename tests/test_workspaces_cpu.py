@@ -181,3 +181,14 @@ def test_calls_run_within_their_stream(monkeypatch, name, args):
     with pytest.raises(KeyboardInterrupt):
         getattr(cb, name)(*first, *[x] * (args - len(first)), stream=side, **kw)
     assert log == [[side]]
+
+
+def test_the_default_stream_of_another_device_is_refused():
+    """Its handle is that of this device's default stream: the call would run, on the wrong one."""
+
+    class Stream:
+        device_index, cuda_stream = 1, 0
+
+    assert ops._raw_stream(Stream(), 1) == 0
+    with pytest.raises(ValueError, match="cuda:1.*cuda:0"):
+        ops._raw_stream(Stream(), 0)
