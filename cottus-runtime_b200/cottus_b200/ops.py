@@ -459,12 +459,11 @@ def quantize_fp8(x, *, block_rows=1, out=None, scales=None, stream=None):
     return out, scales
 
 
-def fp8_linear(x, x_scales, weight, weight_scales, *, residual=None, out=None, out_dtype=torch.float16, status=None,
-               stream=None):
+def fp8_linear(x, x_scales, weight, weight_scales, *, residual=None, out=None, out_dtype=None, status=None, stream=None):
     """Block-scaled e4m3 product (cottus_fp8_linear): out = x . weight^T (+ residual), fp32 accumulation.
     x [rows][in] and x_scales from rms_norm or quantize_fp8; weight [out][in] and weight_scales from
     quantize_fp8(block_rows=128); residual [rows][out] fp32 (may be out itself where out is fp32).
-    in a multiple of 16."""
+    in a multiple of 16.  out_dtype: fp32, fp16 or bf16, by default out's, or fp16."""
     if x.dim() != 2 or weight.dim() != 2:
         raise ValueError("x must be [rows][in] and weight [out][in]")
     dev = _device()
@@ -478,7 +477,9 @@ def fp8_linear(x, x_scales, weight, weight_scales, *, residual=None, out=None, o
     if residual is not None:
         p.residual = _operand(residual, "residual", (rows, fout), _ONLY_F32, dev)
     if out is None:
-        out = _new(x, (rows, fout), out_dtype, stream)
+        out = _new(x, (rows, fout), out_dtype or torch.float16, stream)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise TypeError(f"out is {out.dtype}, out_dtype is {out_dtype}")
     p.out = _operand(out, "out", (rows, fout), _DT_WIDE, dev)
     p.rows, p.out_features, p.in_features = _i32(rows, "rows"), _i32(fout, "out"), _i32(fin, "in")
     p.out_dtype = _DT_WIDE[out.dtype]
@@ -565,9 +566,10 @@ def next_tokens(residual, norm_weight, w_head, head_scales, uniforms, *, eps=1e-
     """The end of a decode step (generic_transformer.cpp:369-370 and the argmax of engine.cpp:85-87), from the residual
     stream [n][hidden] fp32 to one token per row: the final rms_norm to e4m3, the vocabulary projection (fp8_linear,
     w_head [vocab][hidden] e4m3 with the scales of quantize_fp8(block_rows=128)) and sample_tokens.  Returns
-    (tokens int32 [n], logits fp32 [n][vocab])."""
+    (tokens int32 [n], logits [n][vocab], fp32 unless a buffer of another type is given)."""
     h, hs = rms_norm(residual, norm_weight, eps=eps, out_dtype=_FP8, stream=stream)
-    logits = fp8_linear(h, hs, w_head, head_scales, out=logits, out_dtype=torch.float32, status=status, stream=stream)
+    logits = fp8_linear(h, hs, w_head, head_scales, out=logits, out_dtype=None if logits is not None else torch.float32,
+                        status=status, stream=stream)
     tokens = sample_tokens(logits, uniforms, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, out=tokens,
                            status=status, stream=stream)
     return tokens, logits
