@@ -238,7 +238,8 @@ inline bool overlap(const Span& a, const Span& b) {
 // Launch that may start while the stream's preceding kernel drains: the
 // kernel calls grid_dependency_wait() before it touches global memory, and
 // only then grid_dependents_launch(), so that whatever follows starts after
-// everything before this kernel is complete.
+// everything before this kernel is complete.  This kernel itself is not: what a
+// follower does before its own wait is hints (prefetches into L2), no reads.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                               Args&&... args) {

@@ -28,16 +28,24 @@
 // in the result.  exp is table-driven (P. Tang, ACM Trans. Math. Softw. 15,
 // 1989): with y = (logit - max) log2(e) / T in two fp32 words and
 // y = k + j / 256 + r, |r| <= 2^-9,  2^y = 2^k 2^(j/256) (1 + q(r)), the table
-// exact to fixed point and the cubic q < 2^-9 in one fp32 word, so a weight is
-// off by 2^-32 of itself.  (A vocabulary of 2^17 near-equal tokens then draws
+// exact to fixed point and the cubic q < 2^-9 in one fp32 word.  A weight is off
+// by 2^-31 of itself (q's rounding to units of 2^-31 is half of that, the fp32
+// roundings of r and q less than the other half) and by its last place, 2^-43
+// or less of the largest.  (A vocabulary of 2^17 near-equal tokens then draws
 // another token than exact arithmetic once in some 10^6 rows.)  exp in fp64
 // took twice the time of everything else together; it serves the settings
 // that fp32 words cannot hold (temperatures beyond 1e-6 or 1e6, infinities).
 //
-// Bounds: for many rows the integer operations of the exponentials and the
-// barriers (256 x 50257 fp16, temperature alone, 39 us; 4 us of HBM); at one
-// row the chain of cluster barriers, about nine with all filters and 1100 cycles
-// each (1 x 32000 11 us).
+// Bounds: latency.  At one row (1 x 32000, all filters, 11 us) no phase has
+// enough work to hide its own; by the clock of the first CTA: set-up and load
+// 1.6 us with the first cluster barrier, the maximum 1.0, counting the distances
+// and adding them up over the cluster 2.0, finding the bin 1.0, gathering 1.0,
+// and by the first CTA alone two sorts 1.0 and the sums, cuts and the draw 1.9
+// (four cluster barriers in all, 0.5 us each with its wait; top_k above 1024
+// and top-p take more of them).  At many rows (256 x 50257 fp16, temperature
+// alone, 39 us; 4 us of HBM) a CTA takes 14 us, 6 of them the exponentials
+// beside those of the SM's other CTA, 2 the load, the rest the maximum, the sums
+// and the walk; and the 512 CTAs are two waves of 296, the second part empty.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -305,7 +305,8 @@ int cottus_o_proj_residual(const cottus_o_proj_params *p, cottus_stream_t stream
  * ---------------------------------------------------------------------- */
 
 /* RMS norm with the residual's addition: h = x (+ residual), residual_out = h,
- * y = h / sqrt(mean(h^2) + eps) * weight per row, in fp32.  Replaces
+ * y = h / sqrt(mean(h^2) + eps) * weight per row, in fp32 (the sum of squares
+ * too: a row with values from some 10^19 on overflows it).  Replaces
  * residualAddCUDA followed by rmsnormCUDA (compute_primitives_cuda.cu:58-89;
  * rmsnormCPU is the same formula).  y is written in out_dtype: fp32, fp16,
  * bf16 (rounded once), or e4m3 with the row groups' scales. */
@@ -344,8 +345,10 @@ int cottus_quantize_fp8(const cottus_quantize_params *p, cottus_stream_t stream)
  * be a normal fp32 number); x in the activation layout, weight ([out][in], as
  * in cottus_o_proj_residual) in the weight layout.  in_features a multiple of
  * 16, any out_features and any number of rows (a decode batch or a prefill
- * chunk).  Replaces gemmCUDA (compute_primitives_cuda.cu:30-55) and, with
- * residual, the residualAddCUDA after it (generic_transformer.cpp:305-325). */
+ * chunk).  The same call gives the same bits; a row's last bits may differ with
+ * the number of rows, which decides how the sum over k is split up.  Replaces
+ * gemmCUDA (compute_primitives_cuda.cu:30-55) and, with residual, the
+ * residualAddCUDA after it (generic_transformer.cpp:305-325). */
 typedef struct {
     const void *x;          /* [rows][in_features] e4m3, 16-B aligned */
     const float *x_scales;  /* [ceil(in_features/128)][rows] */
@@ -375,7 +378,7 @@ int cottus_fp8_linear(const cottus_fp8_linear_params *p, cottus_stream_t stream)
  *      the front candidate always stays;
  *   5. the token is the first one, in index order, at which the running sum
  *      of the kept weights exceeds uniform * their sum.
- * A weight is off by at most 2^-31 of itself or 2^-43 of the largest one, and
+ * A weight is off by at most 2^-31 of itself and 2^-43 of the largest one, and
  * the sums are of 64-bit fixed-point numbers, so a result does not depend on
  * the order of the additions.
  * temperature <= 0 or NaN takes the front candidate.  top_k <= 0, top_p >= 1
