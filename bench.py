@@ -174,6 +174,11 @@ def run_reference(args, rank, world):
     import torch
     if world > 1 and rank != 0:
         return
+    from oracle.oracle import reference_available
+    if not reference_available():
+        print(json.dumps({"impl": "reference", "unavailable": "oracle/_ref/libcottus_ref.so is not there: it is compiled "
+                          "from the reference's sources (make -C oracle ref)"}), flush=True)
+        return
     if args.config in ("qkv_llama3_8b", "oproj_llama3_8b", "attn_block_llama3_8b"):
         fn, metric = {"qkv_llama3_8b": (qkv_reference_rate, "fused QKV+RoPE+append tokens/s"),
                       "oproj_llama3_8b": (oproj_reference_rate, "O-projection+residual tokens/s"),
